@@ -59,6 +59,10 @@ _PROTOS = {
     "ftm_moe_block_prenorm": (_int, [_vp, _i32, _vp, _vp, _vp, C.c_float, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _int,
                                      _vp, _vp, _int, _vp]),
     "ftm_dense_gemv": (_int, [_vp, _vp, _int, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp]),
+    "ftm_fp8_quantize": (_int, [_vp, _vp, _int, _i32, _i32, C.c_int64, _vp, _vp, _vp]),
+    "ftm_fp8_gemm": (_int, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _int, C.c_int64, _vp]),
+    "ftm_fp8_linear": (_int, [_vp, _vp, _int, C.c_int64, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _int, C.c_int64, _vp]),
+    "ftm_logprobs": (_int, [_vp, _vp, _int, _i32, _i32, C.c_int64, _vp, _int, _i32, _vp, _vp, _vp, _vp, _vp, _vp]),
     "ftm_ftw_open": (_int, [C.c_char_p, C.POINTER(_vp)]),
     "ftm_ftw_parse": (_int, [C.c_char_p, C.POINTER(_vp)]),
     "ftm_ftw_close": (None, [_vp]),

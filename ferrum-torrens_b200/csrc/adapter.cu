@@ -28,7 +28,7 @@ const char* const kKindNames[K_NUM_KINDS] = {
     "router_logits", "router_topk", "slot_rewrite", "csr_build", "expert_gate_up", "expert_down", "sum_routes",
     "shared_phase1", "shared_phase2", "cast_bf16",   "combine",  "grouped_gate_up", "grouped_down",
     "permute_act",   "decode_plan",   "ep_pack",         "ep_combine", "prefill_rescale", "dense_gemv",
-    "add_rmsnorm"};
+    "add_rmsnorm", "fp8_quantize", "fp8_gemm", "logprobs"};
 
 }  // namespace
 
@@ -805,6 +805,10 @@ FTM_API int ftm_sync_status(ftm_handle* h, void* stream) {
         cudaMemsetAsync(h->flags + 1, 0, sizeof(int32_t), s);
         return fail(h, FTM_ERR_BAD, "moe: an expert id was outside [0, %d)", h->cfg.experts);
     }
+    if (f[4]) {
+        cudaMemsetAsync(h->flags + 4, 0, sizeof(int32_t), s);
+        return fail(h, FTM_ERR_BAD, "moe: logprobs: a token id was not below the vocabulary's size");
+    }
     return FTM_OK;
 }
 
@@ -1245,6 +1249,113 @@ FTM_API int ftm_dense_gemv(ftm_handle* h, const void* a, int a_dtype, const void
         return fail(h, FTM_ERR_BAD, "moe: dense gemv: packed must be 16-byte aligned and scale 4-byte aligned");
     h->launches += launch_dense_gemv(a, a_dtype, (const uint32_t*)packed_kmajor_i32, (const uint8_t*)scale_kmajor_u8,
                                      (const uint16_t*)global_f16, m, n, k, c, h->sm_count, h->flags + 2, h->ctx(pick(h, stream)));
+    CU(h, cudaGetLastError());
+    return FTM_OK;
+}
+
+// ---- block-scaled 8-bit products ------------------------------------------------------------
+
+static bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+static size_t act_bytes(int dtype) { return dtype == FTM_BF16 ? 2 : 4; }
+
+static int check_fp8_rows(const ftm_handle* h, const char* what, const void* x, int x_dtype, int64_t rows, int64_t k, int64_t stride) {
+    if (x_dtype != FTM_BF16 && x_dtype != FTM_F32) return fail(h, FTM_ERR_BAD, "moe: %s: activations cannot be dtype %d", what, x_dtype);
+    if (rows <= 0 || k <= 0 || k % 16) return fail(h, FTM_ERR_BAD, "moe: %s: %lld rows of %lld (a nonzero multiple of 16)", what, (long long)rows, (long long)k);
+    if (stride < k) return fail(h, FTM_ERR_BAD, "moe: %s: rows of %lld are %lld apart", what, (long long)k, (long long)stride);
+    if (!aligned_to(x, act_bytes(x_dtype))) return fail(h, FTM_ERR_BAD, "moe: %s: activations not aligned to their type", what);
+    return FTM_OK;
+}
+
+static int check_fp8_weight(const ftm_handle* h, const char* what, const void* w, const float* w_scale, int64_t n, const void* c, int c_dtype,
+                            int64_t c_stride) {
+    if (n <= 0) return fail(h, FTM_ERR_BAD, "moe: %s: %lld weight rows", what, (long long)n);
+    if (c_dtype != FTM_BF16 && c_dtype != FTM_F32) return fail(h, FTM_ERR_BAD, "moe: %s: the output cannot be dtype %d", what, c_dtype);
+    if (c_stride < n) return fail(h, FTM_ERR_BAD, "moe: %s: output rows of %lld are %lld apart", what, (long long)n, (long long)c_stride);
+    if (!aligned_to(w, 16)) return fail(h, FTM_ERR_BAD, "moe: %s: the weight must be 16-byte aligned", what);
+    if (!aligned_to(w_scale, 4) || !aligned_to(c, act_bytes(c_dtype)))
+        return fail(h, FTM_ERR_BAD, "moe: %s: weight scales or output not aligned to their type", what);
+    return FTM_OK;
+}
+
+static int check_fp8_codes(const ftm_handle* h, const char* what, const void* q, const float* scale) {
+    if (!aligned_to(q, 16)) return fail(h, FTM_ERR_BAD, "moe: %s: the codes must be 16-byte aligned", what);
+    if (!aligned_to(scale, 4)) return fail(h, FTM_ERR_BAD, "moe: %s: scales not aligned to their type", what);
+    return FTM_OK;
+}
+
+FTM_API int ftm_fp8_quantize(ftm_handle* h, const void* x, int x_dtype, int32_t rows, int32_t k, int64_t x_stride, void* q_e4m3, float* scale,
+                             void* stream) {
+    if (!h) return FTM_ERR_BAD;
+    std::lock_guard<std::mutex> lk(h->mu);
+    DeviceGuard dg(h->cfg.ordinal);
+    if (!x || !q_e4m3 || !scale) return fail(h, FTM_ERR_BAD, "moe: fp8 quantize: null buffer");
+    int rc = check_fp8_rows(h, "fp8 quantize", x, x_dtype, rows, k, x_stride);
+    if (rc == FTM_OK) rc = check_fp8_codes(h, "fp8 quantize", q_e4m3, scale);
+    if (rc != FTM_OK) return rc;
+    h->launches += launch_fp8_quantize(x, x_dtype, rows, k, x_stride, (uint8_t*)q_e4m3, scale, h->ctx(pick(h, stream)));
+    CU(h, cudaGetLastError());
+    return FTM_OK;
+}
+
+FTM_API int ftm_fp8_gemm(ftm_handle* h, const void* a_e4m3, const float* a_scale, const void* w_e4m3, const float* w_scale, int32_t m, int32_t n,
+                         int32_t k, void* c, int c_dtype, int64_t c_stride, void* stream) {
+    if (!h) return FTM_ERR_BAD;
+    std::lock_guard<std::mutex> lk(h->mu);
+    DeviceGuard dg(h->cfg.ordinal);
+    if (!a_e4m3 || !a_scale || !w_e4m3 || !w_scale || !c) return fail(h, FTM_ERR_BAD, "moe: fp8 gemm: null buffer");
+    if (m <= 0 || k <= 0 || k % 16) return fail(h, FTM_ERR_BAD, "moe: fp8 gemm: %d rows of %d (a nonzero multiple of 16)", m, k);
+    int rc = check_fp8_codes(h, "fp8 gemm", a_e4m3, a_scale);
+    if (rc == FTM_OK) rc = check_fp8_weight(h, "fp8 gemm", w_e4m3, w_scale, n, c, c_dtype, c_stride);
+    if (rc != FTM_OK) return rc;
+    h->launches += launch_fp8_gemm((const uint8_t*)a_e4m3, a_scale, (const uint8_t*)w_e4m3, w_scale, m, n, k, c, c_dtype, c_stride,
+                                   h->ctx(pick(h, stream)));
+    CU(h, cudaGetLastError());
+    return FTM_OK;
+}
+
+FTM_API int ftm_fp8_linear(ftm_handle* h, const void* x, int x_dtype, int64_t x_stride, const void* w_e4m3, const float* w_scale, int32_t m,
+                           int32_t n, int32_t k, void* q_scratch, float* scale_scratch, void* c, int c_dtype, int64_t c_stride, void* stream) {
+    if (!h) return FTM_ERR_BAD;
+    std::lock_guard<std::mutex> lk(h->mu);
+    DeviceGuard dg(h->cfg.ordinal);
+    if (!x || !w_e4m3 || !w_scale || !c) return fail(h, FTM_ERR_BAD, "moe: fp8 linear: null buffer");
+    int rc = check_fp8_rows(h, "fp8 linear", x, x_dtype, m, k, x_stride);
+    if (rc == FTM_OK) rc = check_fp8_weight(h, "fp8 linear", w_e4m3, w_scale, n, c, c_dtype, c_stride);
+    if (rc != FTM_OK) return rc;
+    if (!q_scratch || !scale_scratch) return fail(h, FTM_ERR_BAD, "moe: fp8 linear: %d rows of %d need scratch for their codes and scales", m, k);
+    rc = check_fp8_codes(h, "fp8 linear", q_scratch, scale_scratch);
+    if (rc != FTM_OK) return rc;
+    const Ctx ctx = h->ctx(pick(h, stream));
+    h->launches += launch_fp8_quantize(x, x_dtype, m, k, x_stride, (uint8_t*)q_scratch, scale_scratch, ctx);
+    h->launches += launch_fp8_gemm((const uint8_t*)q_scratch, scale_scratch, (const uint8_t*)w_e4m3, w_scale, m, n, k, c, c_dtype, c_stride, ctx);
+    CU(h, cudaGetLastError());
+    return FTM_OK;
+}
+
+// ---- what a server reads off its logits -----------------------------------------------------
+
+FTM_API int ftm_logprobs(ftm_handle* h, const void* logits, int dtype, int32_t rows, int32_t vocab, int64_t row_stride, const void* ids,
+                         int ids_dtype, int32_t top_n, float* logprob_out, float* entropy_out, int32_t* rank_out, int32_t* top_ids_out,
+                         float* top_logprobs_out, void* stream) {
+    if (!h) return FTM_ERR_BAD;
+    std::lock_guard<std::mutex> lk(h->mu);
+    DeviceGuard dg(h->cfg.ordinal);
+    if (!logits) return fail(h, FTM_ERR_BAD, "moe: logprobs: null buffer");
+    if (dtype != FTM_BF16 && dtype != FTM_F32) return fail(h, FTM_ERR_BAD, "moe: logprobs: logits cannot be dtype %d", dtype);
+    if (rows <= 0 || vocab <= 0 || vocab > (1 << 30)) return fail(h, FTM_ERR_BAD, "moe: logprobs: %d rows of %d logits", rows, vocab);
+    if (row_stride < vocab) return fail(h, FTM_ERR_BAD, "moe: logprobs: rows of %d are %lld apart", vocab, (long long)row_stride);
+    if (ids && ids_dtype != FTM_I32 && ids_dtype != FTM_I64) return fail(h, FTM_ERR_BAD, "moe: logprobs: token ids cannot be dtype %d", ids_dtype);
+    if (!ids && (logprob_out || rank_out)) return fail(h, FTM_ERR_BAD, "moe: logprobs: a log probability or rank needs token ids");
+    if (top_n < 0 || top_n > 32) return fail(h, FTM_ERR_BAD, "moe: logprobs: %d alternatives (at most 32)", top_n);
+    if (top_n && (!top_ids_out || !top_logprobs_out)) return fail(h, FTM_ERR_BAD, "moe: logprobs: null buffer for the alternatives");
+    if (!logprob_out && !entropy_out && !rank_out && !top_n) return fail(h, FTM_ERR_BAD, "moe: logprobs: nothing is asked for");
+    if (!aligned_to(logits, act_bytes(dtype)) || !aligned_to(ids, ids_dtype == FTM_I64 ? 8 : 4) || !aligned_to(logprob_out, 4) ||
+        !aligned_to(entropy_out, 4) || !aligned_to(rank_out, 4) || !aligned_to(top_ids_out, 4) || !aligned_to(top_logprobs_out, 4))
+        return fail(h, FTM_ERR_BAD, "moe: logprobs: a buffer is not aligned to its type");
+    const int n = launch_logprobs(logits, dtype, rows, vocab, row_stride, ids, ids_dtype, top_n, logprob_out, entropy_out, rank_out, top_ids_out,
+                                  top_logprobs_out, h->sm_total, h->flags + 4, h->ctx(pick(h, stream)));
+    if (n < 0) return cuda_fail(h, (cudaError_t)-n, "logprobs");
+    h->launches += n;
     CU(h, cudaGetLastError());
     return FTM_OK;
 }

@@ -31,6 +31,9 @@ enum Kind {
     K_PREFILL_RESCALE,
     K_DENSE_GEMV,
     K_ADD_RMSNORM,
+    K_FP8_QUANTIZE,
+    K_FP8_GEMM,
+    K_LOGPROBS,
     K_NUM_KINDS
 };
 
@@ -252,5 +255,15 @@ int launch_add_rmsnorm(const __nv_bfloat16* x, const __nv_bfloat16* r, const __n
 bool dense_gemv_supported(int N, int K);
 int launch_dense_gemv(const void* a, int a_dtype, const uint32_t* packed, const uint8_t* scale, const uint16_t* global,
                       int M, int N, int K, float* c, int sm_count, int32_t* err, const Ctx& ctx);
+
+// fp8.cu: block-scaled 8-bit products and the quantisation of their activations
+int launch_fp8_quantize(const void* x, int x_dtype, int rows, int K, long long stride, uint8_t* q, float* scale, const Ctx& c);
+int launch_fp8_gemm(const uint8_t* a, const float* a_scale, const uint8_t* w, const float* w_scale, int M, int N, int K, void* out,
+                    int out_dtype, long long ldc, const Ctx& c);
+
+// logprobs.cu: what a server reads off its logits; a negative result is a CUDA error code
+int launch_logprobs(const void* logits, int dtype, int rows, int vocab, long long stride, const void* ids, int ids_dtype, int top_n,
+                    float* logprob, float* entropy, int32_t* rank, int32_t* top_ids, float* top_logprobs, int sm_count,
+                    int32_t* bad_flag, const Ctx& c);
 
 }  // namespace ftm

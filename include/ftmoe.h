@@ -257,6 +257,43 @@ FTM_API int ftm_moe_block_prenorm(ftm_handle* h, int32_t layer, const void* attn
 FTM_API int ftm_dense_gemv(ftm_handle* h, const void* a, int a_dtype, const void* packed_kmajor_i32, const void* scale_kmajor_u8,
                            const void* global_f16, int32_t m, int32_t n, int32_t k, float* c, void* stream);
 
+/* ---- block-scaled 8-bit products (no counterpart in the reference; its 8-bit projections keep 16-bit activations) -- */
+/* Activations to e4m3 with one scale for each row and block of 128 elements (the last block may be shorter):
+ *   a0 = max(largest magnitude of the block, 448 * 2^-126),  scale = a0 / 448,  q = e4m3(x * (448 / a0))
+ * in f32, rounded to the nearest code, ties to even; a NaN stays one and does not count as a magnitude, a block with an
+ * infinity has scale infinity and codes 0 and NaN.  x [rows, k] bf16 or f32 dev, its rows x_stride elements apart;
+ * q [rows, k] e4m3 dev, 16-byte aligned; scale [ceil(k / 128), rows] f32 dev.  k a multiple of 16.  Asynchronous. */
+FTM_API int ftm_fp8_quantize(ftm_handle* h, const void* x, int x_dtype, int32_t rows, int32_t k, int64_t x_stride, void* q_e4m3,
+                             float* scale, void* stream);
+/* c[t, n] = sum over blocks b of 128 k of  a_scale[b, t] * w_scale[n / 128, b] * sum_{k in b} a[t, k] * w[n, k],
+ * every sum in f32, c rounded once.  a [m, k] and a_scale as ftm_fp8_quantize writes them; w [n, k] e4m3 dev and w_scale
+ * [ceil(n / 128), ceil(k / 128)] f32 dev, the layout of checkpoints in 8 bits; a and w 16-byte aligned.  c [m, n] bf16 or
+ * f32 dev, its rows c_stride elements apart (what lies between n and c_stride is not written).  k a multiple of 16, any
+ * m and n.  The same inputs give the same bits.  Asynchronous. */
+FTM_API int ftm_fp8_gemm(ftm_handle* h, const void* a_e4m3, const float* a_scale, const void* w_e4m3, const float* w_scale, int32_t m,
+                         int32_t n, int32_t k, void* c, int c_dtype, int64_t c_stride, void* stream);
+/* ftm_fp8_gemm of ftm_fp8_quantize(x) in one call.  q_scratch [m, k] (16-byte aligned) and scale_scratch
+ * [ceil(k / 128), m] f32 are the caller's, so calls that overlap on the GPU do not meet in them.  Asynchronous. */
+FTM_API int ftm_fp8_linear(ftm_handle* h, const void* x, int x_dtype, int64_t x_stride, const void* w_e4m3, const float* w_scale,
+                           int32_t m, int32_t n, int32_t k, void* q_scratch, float* scale_scratch, void* c, int c_dtype,
+                           int64_t c_stride, void* stream);
+
+/* ---- what a server reads off its logits (no counterpart in the reference) ------------------------------------ */
+/* logits [rows, vocab] bf16 or f32 dev, rows row_stride elements apart (as ftm_dense_gemv or ftm_fp8_linear leave them);
+ * ids [rows] i32 or i64 dev, one token per row.  Per row, with all sums in f32:
+ *   logprob_out   log softmax(logits)[id]
+ *   entropy_out   -sum p log p  (an element of -inf adds nothing)
+ *   rank_out      how many elements come before the token in the order (value descending, index ascending)
+ *   top_ids_out, top_logprobs_out [rows, top_n]   the first top_n (at most 32) elements of that order and their log probabilities
+ * A negative id asks for nothing: logprob 0, rank -1.  An id of vocab or more: logprob NaN, rank -1, and ftm_sync_status
+ * reports it.  A row that is -inf throughout: log probabilities -inf, entropy 0.  A row with a NaN or +inf: NaN for
+ * logprob, entropy and top_logprobs; in the order a NaN counts as -inf.  Places past the vocabulary: id -1, -inf.
+ * Each output may be NULL (ids too when neither logprob nor rank is wanted; top_n 0 leaves out the alternatives).
+ * Asynchronous; no scratch, so calls on several streams do not meet. */
+FTM_API int ftm_logprobs(ftm_handle* h, const void* logits, int dtype, int32_t rows, int32_t vocab, int64_t row_stride, const void* ids,
+                         int ids_dtype, int32_t top_n, float* logprob_out, float* entropy_out, int32_t* rank_out, int32_t* top_ids_out,
+                         float* top_logprobs_out, void* stream);
+
 /* ---- FTW checkpoint: index and expert banks ---------------------------------------------------
  * The checkpoint the reference engine loads (src/infrastructure/ftw.rs): a JSON index
  * `freetoken_weight.json` over one logical byte region cut into shard files.  Host code only; none of

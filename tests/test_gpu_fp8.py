@@ -1,0 +1,301 @@
+"""The block-scaled 8-bit products (fp8_quantize, fp8_gemm, fp8_linear) against their formulas in 64 bits."""
+import ctypes as C
+import importlib
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+pkg = importlib.import_module("ferrum-torrens_b200")
+L = pkg._lib
+
+E4M3 = torch.float8_e4m3fn
+DT = {"bf16": torch.bfloat16, "f32": torch.float32}
+DEV = "cuda:0"
+
+
+@pytest.fixture(scope="module")
+def moe():
+    m = pkg.B200MoE(0, pkg.ExpertShapes(64, 16), 1, experts=1, layers=1, top_k=1, shared_inter=16, max_tokens=1)
+    yield m
+    m.close()
+
+
+def rng(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def activations(seed, m, k, dtype, pad=0, offset=0):
+    """[m, k] whose rows are k + pad apart and start `offset` elements into their buffer."""
+    buf = torch.randn((m, k + pad), generator=rng(seed), device=DEV) * torch.exp2(3 * torch.randn((m, 1), generator=rng(seed + 1), device=DEV))
+    return buf.to(dtype)[:, offset:offset + k]
+
+
+def weight(seed, n, k):
+    w = (torch.randn((n, k), generator=rng(seed), device=DEV) * 90).clamp(-448, 448).to(E4M3)
+    s = torch.exp2(torch.randn((-(-n // 128), -(-k // 128)), generator=rng(seed + 7), device=DEV)) * 1e-3
+    return w, s
+
+
+# ------------------------------------------------------------------ the formulas, in 64 bits on the CPU
+def e4m3_nearest(y):
+    """The e4m3 value nearest to each y, ties to even, saturating."""
+    step = np.exp2(np.floor(np.log2(np.maximum(np.abs(y), 2.0 ** -6))) - 3)
+    return np.clip(np.round(y / step) * step, -448, 448)
+
+
+def quantised(x):
+    """(codes' values [M, K], scales [blocks, M]): the three roundings to f32 are the definition's."""
+    x = x.double().cpu().numpy()
+    m, k = x.shape
+    q, scales = np.zeros((m, k)), []
+    with np.errstate(invalid="ignore", over="ignore"):
+        for b in range(0, k, 128):
+            v = x[:, b:b + 128]
+            a0 = np.maximum(np.nan_to_num(np.abs(v), nan=0.0, posinf=np.inf).max(1), 448 * 2.0 ** -126).astype(np.float32).astype(np.float64)
+            inv = (448.0 / a0).astype(np.float32).astype(np.float64)
+            y = (v * inv[:, None]).astype(np.float32).astype(np.float64)
+            q[:, b:b + 128] = np.where(np.isnan(y), np.nan, e4m3_nearest(np.nan_to_num(y)))
+            scales.append((a0 / 448.0).astype(np.float32))
+    return q, np.stack(scales)
+
+
+def product(q, scales, w, ws):
+    """(c, S) in 64 bits: S the sum of the terms' magnitudes, which the rounding errors go by."""
+    w, ws = w.float().double().cpu().numpy(), ws.double().cpu().numpy()
+    c, mag = 0.0, 0.0
+    for b in range(scales.shape[0]):
+        at = slice(128 * b, 128 * b + 128)
+        rows = q[:, at] * scales[b].astype(np.float64)[:, None]
+        cols = w[:, at] * np.repeat(ws[:, b], 128)[:w.shape[0], None]
+        c, mag = c + rows @ cols.T, mag + np.abs(rows) @ np.abs(cols).T
+    return c, mag
+
+
+def check_product(got, q, scales, w, ws):
+    c, mag = product(q, scales, w, ws)
+    blocks = scales.shape[0]
+    # products of e4m3 are exact in f32; 128 additions of a block, one per block, the product of the two scales and its
+    # multiplication: each off by at most one step 2^-23 (a tensor core may cut off where an ALU rounds)
+    tol = (128 + blocks + 3) * 2.0 ** -23 * mag + np.abs(c) * torch.finfo(got.dtype).eps / 2 + 1e-38
+    d = np.abs(got.double().cpu().numpy() - c)
+    assert (d <= tol).all(), (float((d / tol).max()), np.unravel_index(np.argmax(d / tol), d.shape))
+
+
+# ------------------------------------------------------------------ quantisation
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("m,k,pad,offset", [(1, 16, 0, 0), (1, 128, 0, 0), (2, 144, 0, 0), (7, 1040, 16, 8), (37, 2048, 0, 0), (9, 2000, 5, 3),
+                                            (8, 256, 1, 1), (300, 4096, 0, 0), (1, 16, 1, 1)])
+def test_quantize_is_the_formula_bit_for_bit(moe, m, k, pad, offset, dtype):
+    x = activations(m * 1000 + k, m, k, DT[dtype], pad, offset)
+    q, s = moe.fp8_quantize(x)
+    want_q, want_s = quantised(x)
+    assert np.array_equal(s.cpu().numpy(), want_s)
+    assert np.array_equal(q.float().cpu().numpy(), want_q.astype(np.float32))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_quantize_special_values(moe, dtype):
+    big, tiny = torch.finfo(DT[dtype]).max, torch.finfo(DT[dtype]).smallest_normal
+    rows = torch.zeros((8, 272))
+    rows[0] = 0.0
+    rows[1] = tiny / 4                                   # all subnormal
+    rows[2, ::3], rows[2, 5] = big, -big
+    rows[3] = torch.arange(272) - 135.5
+    rows[4] = 1.0
+    rows[4, 7], rows[4, 130] = float("nan"), float("nan")     # a NaN is one element's matter
+    rows[5] = 2.0
+    rows[5, 3] = float("inf")                            # an infinity is its block's
+    rows[5, 4] = float("-inf")
+    rows[6, :128] = 448.0
+    rows[6, :16] = torch.tensor([17., 18., 19., 20., 21., 22., 23., 1.0625, 1.1875, 2.0 ** -10, 3 * 2.0 ** -10, 2.0 ** -9, 447., 432., 440., -0.0])
+    rows[7, 128:] = -tiny
+    x = rows.to(DT[dtype]).to(DEV)
+    q, s = moe.fp8_quantize(x)
+    want_q, want_s = quantised(x)
+    assert np.array_equal(s.cpu().numpy(), want_s)
+    assert np.array_equal(q.float().cpu().numpy(), want_q.astype(np.float32), equal_nan=True)
+    assert np.isinf(want_s[0, 5]) and np.isnan(want_q[5, 3:5]).all() and (want_q[5, 5:128] == 0).all()
+    assert want_s[0, 0] == 2.0 ** -126
+
+
+def test_quantize_writes_its_rows_only_and_reaches_past_32_bits(moe):
+    m, k = 2 ** 20 + 3, 2048
+    x = torch.empty((m, k), dtype=torch.bfloat16, device=DEV)
+    x[-3:] = activations(5, 3, k, torch.bfloat16)
+    x[:3] = x[-3:]
+    q = torch.empty((m + 2, k), dtype=torch.uint8, device=DEV)
+    q[-2:] = 0xa5
+    s = torch.full((16 * m + 5,), -7.0, device=DEV)
+    moe.fp8_quantize(x, out=(q[:m].view(E4M3), s[:16 * m].view(16, m)))
+    want_q, want_s = quantised(x[-3:])
+    assert np.array_equal(q[m - 3:m].view(E4M3).float().cpu().numpy(), want_q.astype(np.float32))
+    assert np.array_equal(s[:16 * m].view(16, m)[:, -3:].cpu().numpy(), want_s)
+    assert (q[-2:] == 0xa5).all() and (s[16 * m:] == -7.0).all()
+
+
+# ------------------------------------------------------------------ products
+SHAPES = [(1, 1, 16), (1, 128, 128), (2, 129, 144), (3, 5, 4112), (8, 2048, 512), (15, 640, 2048), (16, 64, 2048), (16, 300, 8192), (17, 130, 272),
+          (31, 1000, 128), (33, 300, 1040), (64, 512, 512), (65, 257, 2048), (100, 2048, 4096), (127, 127, 112), (128, 128, 128), (129, 384, 640),
+          (200, 1000, 2000), (256, 256, 256), (300, 4100, 400), (513, 768, 1152), (1000, 2050, 2064), (2100, 520, 384)]
+
+
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_gemm(moe, m, n, k, out):
+    q, s = moe.fp8_quantize(activations(m + n, m, k, torch.float32))
+    w, ws = weight(k + n, n, k)
+    buf = torch.full((m + 1, n + 3), 77.0, dtype=DT[out], device=DEV)
+    c = buf[:m, :n]                                      # rows apart; what is behind a row and behind the last row stays
+    moe.fp8_gemm(q, s, w, ws, c)
+    check_product(c, q.double().cpu().numpy(), s.cpu().numpy(), w, ws)
+    assert (buf[:, n:] == 77.0).all() and (buf[m] == 77.0).all()
+    again = torch.empty((m, n), dtype=DT[out], device=DEV)
+    moe.fp8_gemm(q, s, w, ws, again)
+    assert torch.equal(again, c), "the same inputs give the same bits"
+    moe.sync_status()
+
+
+@pytest.mark.parametrize("x,out", [("bf16", "bf16"), ("bf16", "f32"), ("f32", "bf16"), ("f32", "f32")])
+@pytest.mark.parametrize("m,n,k,pad,offset", [(1, 2048, 2048, 0, 0), (1, 1, 16, 0, 0), (4, 300, 2000, 8, 0), (7, 1025, 4096, 3, 1), (13, 256, 144, 0, 0),
+                                              (16, 5000, 512, 0, 0), (16, 136, 8192, 0, 0), (5, 200, 8208, 0, 0), (17, 520, 1024, 0, 0), (64, 384, 2048, 8, 8),
+                                              (140, 260, 640, 1, 0)])
+def test_linear_is_the_product_of_the_quantised_rows(moe, m, n, k, pad, offset, x, out):
+    rows = activations(m + 3 * k, m, k, DT[x], pad, offset)
+    w, ws = weight(n, n, k)
+    buf = torch.full((m + 1, n + 5), 77.0, dtype=DT[out], device=DEV)
+    c = moe.fp8_linear(rows, w, ws, buf[:m, :n])
+    q, s = quantised(rows)
+    check_product(c, q, s, w, ws)
+    assert (buf[:, n:] == 77.0).all() and (buf[m] == 77.0).all()
+    again = torch.empty((m, n), dtype=DT[out], device=DEV)
+    scratch = (torch.empty((m, k), dtype=E4M3, device=DEV), torch.empty((-(-k // 128), m), device=DEV))
+    moe.fp8_linear(rows, w, ws, again, scratch=scratch)
+    assert torch.equal(again, c)
+    moe.sync_status()
+
+
+@pytest.mark.parametrize("m", [1, 9, 40, 130, 600])
+def test_special_codes_stay_in_their_row_or_column(moe, m):
+    n, k = 300, 400
+    x = activations(3, m, k, torch.bfloat16)
+    w, ws = weight(4, n, k)
+    clean = torch.empty((m, n), dtype=torch.float32, device=DEV)
+    moe.fp8_linear(x, w, ws, clean)
+    wb = w.clone().view(torch.uint8)
+    wb[77, 399] = 0x7f                                   # NaN code in the last, short block
+    wb[78] = 0x80                                        # a row of -0
+    ws2 = ws.clone()
+    ws2[2, 1] = 0.0
+    x2 = x.clone()
+    x2[m // 2, 130] = float("inf")
+    got = torch.empty_like(clean)
+    moe.fp8_linear(x2, wb.view(E4M3), ws2, got)
+    got, clean = got.cpu().numpy(), clean.cpu().numpy()
+    assert np.isnan(got[:, 77]).all() and np.isnan(got[m // 2]).all()
+    keep = [r for r in range(m) if r != m // 2]
+    assert (got[keep, 78] == 0).all()
+    cols = [j for j in range(256) if j not in (77, 78)]
+    assert np.array_equal(got[np.ix_(keep, cols)], clean[np.ix_(keep, cols)])
+    assert np.isfinite(got[keep][:, 256:]).all()
+
+
+@pytest.mark.parametrize("m", [4, 40, 200])
+def test_largest_codes_and_scales(moe, m):
+    """Sums of 448 * 448 terms, and scales whose product leaves f32's range only where the result does."""
+    n, k = 140, 2048
+    x = torch.full((m, k), 3.0e38, device=DEV)
+    x[:, ::2] *= -1.0
+    x[:, 0] = 3.0e38
+    w = torch.full((n, k), 448.0, device=DEV).to(E4M3)
+    ws = torch.full((2, 16), 1e-30, device=DEV)
+    c = torch.empty((m, n), device=DEV)
+    moe.fp8_linear(x, w, ws, c)
+    q, s = quantised(x)
+    check_product(c, q, s, w, ws)
+
+
+def test_gemm_output_rows_past_32_bits(moe):
+    m, n, k, ld = 9, 64, 128, 2 ** 28 + 1
+    q, s = moe.fp8_quantize(activations(1, m, k, torch.bfloat16))
+    w, ws = weight(2, n, k)
+    buf = torch.empty((8 * ld + n,), dtype=torch.bfloat16, device=DEV)
+    c = buf.as_strided((m, n), (ld, 1))
+    moe.fp8_gemm(q, s, w, ws, c)
+    check_product(c, q.double().cpu().numpy(), s.cpu().numpy(), w, ws)
+
+
+def test_graphs_streams_and_chained_calls(moe):
+    """Captured and replayed on new inputs, twice at once on two streams, and quantise -> product without a wait between."""
+    m, n, k = 12, 1000, 2048
+    w, ws = weight(1, n, k)
+    w2, ws2 = weight(2, 300, 1008)
+    inputs = [activations(i, m, k, torch.bfloat16).contiguous() for i in range(4)]
+
+    def want(x):
+        c = torch.empty((m, n), device=DEV)
+        moe.fp8_linear(x, w, ws, c)
+        return c
+    wanted = [want(x) for x in inputs]
+    x, c = inputs[0].clone(), torch.empty((m, n), device=DEV)
+    y, big = activations(9, 300, 1008, torch.float32), torch.empty((300, 300), dtype=torch.bfloat16, device=DEV)
+    scratch = tuple(t.clone() for t in moe.fp8_quantize(y))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        moe.fp8_linear(x, w, ws, c, scratch=tuple(t.clone() for t in moe.fp8_quantize(x)))
+        moe.fp8_quantize(y, out=scratch)
+        moe.fp8_gemm(*scratch, w2, ws2, big)
+    for i in (1, 2, 3):
+        x.copy_(inputs[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(c, wanted[i])
+    q, s = quantised(y)
+    check_product(big, q, s, w2, ws2)
+    streams, outs = [torch.cuda.Stream() for _ in range(3)], [torch.empty((m, n), device=DEV) for _ in range(3)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for st, x_in, o in zip(streams, inputs, outs):
+            with torch.cuda.stream(st):
+                moe.fp8_linear(x_in, w, ws, o)
+    torch.cuda.synchronize()
+    for o, v in zip(outs, wanted):
+        assert torch.equal(o, v)
+    moe.sync_status()
+
+
+def test_refusals(moe):
+    x = torch.zeros((4, 256), dtype=torch.bfloat16, device=DEV)
+    w, ws = weight(0, 130, 256)
+    q, s = moe.fp8_quantize(x)
+    c = torch.empty((4, 130), device=DEV)
+    bad = [
+        lambda: moe.fp8_quantize(x.half()), lambda: moe.fp8_quantize(x[:, :250]), lambda: moe.fp8_quantize(x.cpu()), lambda: moe.fp8_quantize(x[0]),
+        lambda: moe.fp8_quantize(x.t()), lambda: moe.fp8_quantize(x[:0]), lambda: moe.fp8_quantize(x[:, :0]), lambda: moe.fp8_quantize(x[:1].expand(4, 256)),
+        lambda: moe.fp8_quantize(x, out=(q, s.t().contiguous())), lambda: moe.fp8_quantize(x, out=(q.view(torch.uint8), s)),
+        lambda: moe.fp8_gemm(q, s, w, ws[:1].contiguous(), c), lambda: moe.fp8_gemm(q, s, w[:, :240].contiguous(), ws, c),
+        lambda: moe.fp8_gemm(q, s[:1].contiguous(), w, ws, c), lambda: moe.fp8_gemm(q, s, w, ws.bfloat16(), c), lambda: moe.fp8_gemm(q, s, w, ws, c.half()),
+        lambda: moe.fp8_gemm(q, s, w, ws, c[:3]), lambda: moe.fp8_gemm(q, s, w, ws, c.t()), lambda: moe.fp8_gemm(q, s, w, ws, c[:1].expand(4, 130)),
+        lambda: moe.fp8_gemm(x, s, w, ws, c), lambda: moe.fp8_gemm(q, s, w.t(), ws, c), lambda: moe.fp8_linear(x.cpu(), w, ws, c),
+        lambda: moe.fp8_linear(x, w, ws, c, scratch=(q[:2].contiguous(), s)), lambda: moe.fp8_linear(x[:, :128], w, ws, c),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(pkg.MoEError) as e:
+            call()
+        assert e.value.kind == "Bad", i
+    lib, h, p = L.lib(), moe._h, lambda t, off=0: C.c_void_p(t.data_ptr() + off)
+    null, st = C.c_void_p(0), C.c_void_p(0)
+    gemm = lambda a=p(q), sa=p(s), pw=p(w), sw=p(ws), m=4, n=130, k=256, pc=p(c), dt=L.F32, ld=130: lib.ftm_fp8_gemm(h, a, sa, pw, sw, m, n, k, pc, dt, ld, st)
+    assert gemm() == L.OK
+    for kw in (dict(a=null), dict(sa=null), dict(pw=null), dict(sw=null), dict(pc=null), dict(m=0), dict(m=-1), dict(n=0), dict(k=0), dict(k=248), dict(k=-16),
+               dict(dt=L.I32), dict(ld=129), dict(a=p(q, 8)), dict(pw=p(w, 1)), dict(pc=p(c, 2)), dict(sa=p(s, 2)), dict(sw=p(ws, 1))):
+        assert gemm(**kw) == L.ERR_BAD, kw
+    quant = lambda px=p(x), dt=L.BF16, m=4, k=256, ld=256, pq=p(q), ps=p(s): lib.ftm_fp8_quantize(h, px, dt, m, k, ld, pq, ps, st)
+    assert quant() == L.OK
+    for kw in (dict(px=null), dict(pq=null), dict(ps=null), dict(dt=L.I64), dict(m=0), dict(k=8), dict(ld=255), dict(px=p(x, 1)), dict(pq=p(q, 4)), dict(ps=p(s, 1))):
+        assert quant(**kw) == L.ERR_BAD, kw
+    assert lib.ftm_fp8_gemm(null, null, null, null, null, 1, 1, 16, null, 0, 1, null) == L.ERR_BAD
+    torch.cuda.synchronize()
