@@ -1255,6 +1255,14 @@ FTM_API int ftm_dense_gemv(ftm_handle* h, const void* a, int a_dtype, const void
 
 // ---- block-scaled 8-bit products ------------------------------------------------------------
 
+// what a launcher answers: kernels launched, or a CUDA error code below zero
+static int count_launches(ftm_handle* h, int n, const char* what) {
+    if (n < 0) return cuda_fail(h, (cudaError_t)-n, what);
+    h->launches += n;
+    CU(h, cudaGetLastError());
+    return FTM_OK;
+}
+
 static bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 static size_t act_bytes(int dtype) { return dtype == FTM_BF16 ? 2 : 4; }
 
@@ -1292,9 +1300,7 @@ FTM_API int ftm_fp8_quantize(ftm_handle* h, const void* x, int x_dtype, int32_t 
     int rc = check_fp8_rows(h, "fp8 quantize", x, x_dtype, rows, k, x_stride);
     if (rc == FTM_OK) rc = check_fp8_codes(h, "fp8 quantize", q_e4m3, scale);
     if (rc != FTM_OK) return rc;
-    h->launches += launch_fp8_quantize(x, x_dtype, rows, k, x_stride, (uint8_t*)q_e4m3, scale, h->ctx(pick(h, stream)));
-    CU(h, cudaGetLastError());
-    return FTM_OK;
+    return count_launches(h, launch_fp8_quantize(x, x_dtype, rows, k, x_stride, (uint8_t*)q_e4m3, scale, h->ctx(pick(h, stream))), "fp8 quantize");
 }
 
 FTM_API int ftm_fp8_gemm(ftm_handle* h, const void* a_e4m3, const float* a_scale, const void* w_e4m3, const float* w_scale, int32_t m, int32_t n,
@@ -1307,10 +1313,8 @@ FTM_API int ftm_fp8_gemm(ftm_handle* h, const void* a_e4m3, const float* a_scale
     int rc = check_fp8_codes(h, "fp8 gemm", a_e4m3, a_scale);
     if (rc == FTM_OK) rc = check_fp8_weight(h, "fp8 gemm", w_e4m3, w_scale, n, c, c_dtype, c_stride);
     if (rc != FTM_OK) return rc;
-    h->launches += launch_fp8_gemm((const uint8_t*)a_e4m3, a_scale, (const uint8_t*)w_e4m3, w_scale, m, n, k, c, c_dtype, c_stride,
-                                   h->ctx(pick(h, stream)));
-    CU(h, cudaGetLastError());
-    return FTM_OK;
+    return count_launches(h, launch_fp8_gemm((const uint8_t*)a_e4m3, a_scale, (const uint8_t*)w_e4m3, w_scale, m, n, k, c, c_dtype, c_stride,
+                                             h->sm_count, h->flags + 2, h->ctx(pick(h, stream))), "fp8 gemm");
 }
 
 FTM_API int ftm_fp8_linear(ftm_handle* h, const void* x, int x_dtype, int64_t x_stride, const void* w_e4m3, const float* w_scale, int32_t m,
@@ -1322,14 +1326,17 @@ FTM_API int ftm_fp8_linear(ftm_handle* h, const void* x, int x_dtype, int64_t x_
     int rc = check_fp8_rows(h, "fp8 linear", x, x_dtype, m, k, x_stride);
     if (rc == FTM_OK) rc = check_fp8_weight(h, "fp8 linear", w_e4m3, w_scale, n, c, c_dtype, c_stride);
     if (rc != FTM_OK) return rc;
+    const Ctx ctx = h->ctx(pick(h, stream));
+    if (fp8_fused_supported(m, k))
+        return count_launches(h, launch_fp8_linear(x, x_dtype, x_stride, (const uint8_t*)w_e4m3, w_scale, m, n, k, c, c_dtype, c_stride, h->sm_count,
+                                                   h->flags + 2, ctx), "fp8 linear");
     if (!q_scratch || !scale_scratch) return fail(h, FTM_ERR_BAD, "moe: fp8 linear: %d rows of %d need scratch for their codes and scales", m, k);
     rc = check_fp8_codes(h, "fp8 linear", q_scratch, scale_scratch);
     if (rc != FTM_OK) return rc;
-    const Ctx ctx = h->ctx(pick(h, stream));
-    h->launches += launch_fp8_quantize(x, x_dtype, m, k, x_stride, (uint8_t*)q_scratch, scale_scratch, ctx);
-    h->launches += launch_fp8_gemm((const uint8_t*)q_scratch, scale_scratch, (const uint8_t*)w_e4m3, w_scale, m, n, k, c, c_dtype, c_stride, ctx);
-    CU(h, cudaGetLastError());
-    return FTM_OK;
+    rc = count_launches(h, launch_fp8_quantize(x, x_dtype, m, k, x_stride, (uint8_t*)q_scratch, scale_scratch, ctx), "fp8 quantize");
+    if (rc != FTM_OK) return rc;
+    return count_launches(h, launch_fp8_gemm((const uint8_t*)q_scratch, scale_scratch, (const uint8_t*)w_e4m3, w_scale, m, n, k, c, c_dtype, c_stride,
+                                             h->sm_count, h->flags + 2, ctx), "fp8 linear");
 }
 
 // ---- what a server reads off its logits -----------------------------------------------------
@@ -1352,12 +1359,8 @@ FTM_API int ftm_logprobs(ftm_handle* h, const void* logits, int dtype, int32_t r
     if (!aligned_to(logits, act_bytes(dtype)) || !aligned_to(ids, ids_dtype == FTM_I64 ? 8 : 4) || !aligned_to(logprob_out, 4) ||
         !aligned_to(entropy_out, 4) || !aligned_to(rank_out, 4) || !aligned_to(top_ids_out, 4) || !aligned_to(top_logprobs_out, 4))
         return fail(h, FTM_ERR_BAD, "moe: logprobs: a buffer is not aligned to its type");
-    const int n = launch_logprobs(logits, dtype, rows, vocab, row_stride, ids, ids_dtype, top_n, logprob_out, entropy_out, rank_out, top_ids_out,
-                                  top_logprobs_out, h->sm_total, h->flags + 4, h->ctx(pick(h, stream)));
-    if (n < 0) return cuda_fail(h, (cudaError_t)-n, "logprobs");
-    h->launches += n;
-    CU(h, cudaGetLastError());
-    return FTM_OK;
+    return count_launches(h, launch_logprobs(logits, dtype, rows, vocab, row_stride, ids, ids_dtype, top_n, logprob_out, entropy_out, rank_out,
+                                             top_ids_out, top_logprobs_out, h->sm_total, h->flags + 4, h->ctx(pick(h, stream))), "logprobs");
 }
 
 }  // extern "C"

@@ -1,0 +1,44 @@
+// Activations to e4m3 with one scale for each row and block of 128 (the formula is in fp8.cuh).
+//
+// Memory bound: one read of x, one write of the codes.  Sixteen lanes own a block, eight elements each, so the block's maximum
+// is four shuffles and x stays in registers.  The eight warps of a CTA take eight rows of the same blocks: the scales of
+// neighbouring rows are neighbours in memory.
+#include "fp8.cuh"
+#include "kernels.cuh"
+
+namespace ftm {
+
+namespace {
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+fp8_quantize_kernel(const T* __restrict__ x, long long stride, int rows, int K, bool vec, uint8_t* __restrict__ q, float* __restrict__ scale) {
+    const int lane = threadIdx.x % 32, blocks = (K + kFp8Block - 1) / kFp8Block;
+    const long long row = (long long)blockIdx.x * 8 + threadIdx.x / 32;
+    if (row >= rows) return;
+    for (int b = blockIdx.y * 2 + lane / 16; b - lane / 16 < blocks; b += gridDim.y * 2) {
+        const int k = b * kFp8Block + (lane % 16) * 8;
+        float f[8], sc;
+        fp8_load8(x + row * stride + k, vec, b < blocks ? K - k : 0, f);
+        const uint2 codes = fp8_encode8(f, sc);
+        if (b < blocks && k < K) *reinterpret_cast<uint2*>(q + row * K + k) = codes;
+        if (b < blocks && lane % 16 == 0) scale[(long long)b * rows + row] = sc;
+    }
+}
+
+}  // namespace
+
+int launch_fp8_quantize(const void* x, int x_dtype, int rows, int K, long long stride, uint8_t* q, float* scale, const Ctx& c) {
+    const int blocks = (K + kFp8Block - 1) / kFp8Block;
+    const bool vec = fp8_rows_aligned(x, x_dtype, stride);
+    const dim3 grid(((unsigned)rows + 7) / 8, min((blocks + 1) / 2, 65535));
+    c.begin(K_FP8_QUANTIZE);
+    if (x_dtype == 0)
+        fp8_quantize_kernel<<<grid, 256, 0, c.s>>>((const __nv_bfloat16*)x, stride, rows, K, vec, q, scale);
+    else
+        fp8_quantize_kernel<<<grid, 256, 0, c.s>>>((const float*)x, stride, rows, K, vec, q, scale);
+    c.end();
+    return 1;
+}
+
+}  // namespace ftm

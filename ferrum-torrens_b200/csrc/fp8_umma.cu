@@ -1,0 +1,418 @@
+// Block-scaled 8-bit products on the tcgen05 tensor cores.
+//
+//   c[t, n] = sum_b (a_scale[b, t] * w_scale[n / 128, b]) * (sum over k in block b of a[t, k] * w[n, k])
+//
+// A tile is 128 weight rows (one block of weight scales, the tensor memory's lanes) by NT tokens (its columns).  A block of 128 k is one
+// 128-byte swizzle atom of either operand and four tcgen05.mma (kind::f8f6f4, exact products, f32 sums) into an accumulator of its own;
+// the epilogue warps read it, multiply every column by its scale and add it to sums in registers.  The scales differ from block to
+// block, so a sum over all of k cannot stay in tensor memory; with two or four accumulators the next blocks are
+// multiplied meanwhile.
+//   warp 0      TMA: weight box [128 rows x 128 k], token box [NT x 128 k]
+//   warp 1      issues the products
+//   warp 2      allocates the tensor memory; multiplies the two scales of every (block, token) ahead of the epilogue
+//   warps 4..   epilogue: four warps for NT <= 32, eight above (each four take half of the columns)
+// Few tiles: the blocks of k are split over the CTAs of a cluster.  Every CTA stores its sums of the tokens that CTA r finishes into r's
+// shared memory, which adds them in the order of the ranks, so the same inputs give the same bits and no scratch in
+// global memory is needed.
+// FUSED (at most 16 tokens): the rows are still bf16 or f32.  The epilogue warps first quantise the CTA's share of them
+// into the swizzled operand layout, while the first weight boxes are on their way; they stay there for all tiles.
+// Every wait is bounded; a wait that gives up raises the error flag and the CTA drains.
+#include "fp8.cuh"
+#include "kernels.cuh"
+#include "umma.cuh"
+
+namespace ftm {
+
+namespace {
+
+using namespace umma;
+
+constexpr int kRows = 128;                       // weight rows of a tile
+constexpr int kWBytes = kRows * kFp8Block;       // a weight box
+constexpr int kMaxStages = 12, kMaxAcc = 4, kMaxSplit = 8;
+constexpr int kBarBytes = 512;
+
+__device__ __forceinline__ void umma_f8_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+// address of the same shared memory in another CTA of the cluster
+__device__ __forceinline__ uint32_t map_shared_to(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void remote_store(uint32_t addr, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+// one arrival of a converged warp on a barrier of another CTA; what its lanes stored before is visible to who waits there
+__device__ __forceinline__ void remote_arrive_warp(uint32_t bar) {
+    asm volatile("fence.acq_rel.cluster;" ::: "memory");
+    __syncwarp();
+    if (threadIdx.x % 32 == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool cluster_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* err) {
+    for (uint32_t i = 0; i < kSpin; i++) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if ((i & 1023u) == 1023u && *abort_flag) return false;
+    }
+    *abort_flag = 1;
+    atomicExch(err, 3);
+    return false;
+}
+
+struct Fp8Args {
+    const void* x;               // FUSED: the rows
+    long long x_stride;
+    int x_dtype, x_vec;
+    const float* a_scale;        // [blocks, M]
+    const float* w_scale;        // [ceil(N / 128), blocks]
+    int M, N, K, blocks;
+    int t_tiles, tiles;          // tiles = t_tiles * ceil(N / 128)
+    int stages;
+    void* c;
+    int c_dtype;
+    long long ldc;
+    int32_t* err;
+};
+
+template <int NT, bool FUSED>
+struct Shape {
+    static constexpr int kEpi = NT >= 64 ? 8 : 4;                // epilogue warps
+    static constexpr int kThreads = 128 + 32 * kEpi;
+    static constexpr int kCols = NT * 4 / kEpi;                  // columns of one epilogue warp
+    static constexpr int kAcc = NT >= 128 ? 2 : 4;               // accumulators (and slots of scales)
+    static constexpr int kTmem = NT * kAcc < 32 ? 32 : NT * kAcc;
+    static constexpr int kABytes = NT * kFp8Block;               // a token box
+    static constexpr int kStage = kWBytes + (FUSED ? 0 : kABytes);
+    // after the ring: sums from the cluster's CTAs [ranks][NT / ranks][128], slots of scales, FUSED: codes and scales of the rows
+    static size_t bytes(int stages, int split, int fused_blocks) {
+        return 1024 + (size_t)stages * kStage + (FUSED ? (size_t)fused_blocks * (kABytes + NT * 4) : 0) + (split > 1 ? (size_t)NT * kRows * 4 : 0) +
+               kAcc * NT * 4 + kBarBytes;
+    }
+};
+
+__device__ __forceinline__ void store_out(const Fp8Args& a, int t, int n, float v) { store_act(a.c, a.c_dtype, (size_t)t * a.ldc + n, v); }
+
+template <int NT, bool FUSED>
+__global__ void __launch_bounds__(Shape<NT, FUSED>::kThreads, 1)
+fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_a, const Fp8Args a, const int split) {
+    using S = Shape<NT, FUSED>;
+    constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(NT >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);   // e4m3 x e4m3 -> f32
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* const ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    const int rank = split > 1 ? (int)cluster_rank() : 0;
+    const int kb0 = a.blocks * rank / split, kb1 = a.blocks * (rank + 1) / split, nkb = kb1 - kb0;
+    const int max_nkb = (a.blocks + split - 1) / split;
+    uint8_t* const codes = ring + (size_t)a.stages * S::kStage;                          // FUSED [max_nkb][NT x 128]
+    float* const sums = reinterpret_cast<float*>(codes + (FUSED ? (size_t)max_nkb * S::kABytes : 0));
+    float* const slots = sums + (split > 1 ? NT * kRows : 0);                            // [kAcc][NT]
+    float* const row_scales = slots + S::kAcc * NT;                                      // FUSED [max_nkb][NT]
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(row_scales + (FUSED ? max_nkb * NT : 0));
+    const uint32_t bar0 = smem_u32(bars);
+    auto FULL = [&](int s) { return bar0 + 8u * s; };
+    auto EMPTY = [&](int s) { return bar0 + 8u * (kMaxStages + s); };
+    auto ACC_FULL = [&](int p) { return bar0 + 8u * (2 * kMaxStages + p); };
+    auto ACC_EMPTY = [&](int p) { return bar0 + 8u * (2 * kMaxStages + kMaxAcc + p); };
+    const uint32_t CODES = bar0 + 8u * (2 * kMaxStages + 2 * kMaxAcc), SUM_FULL = CODES + 8, SUM_FREE = CODES + 16;
+    uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(bars + 2 * kMaxStages + 2 * kMaxAcc + 4);
+    volatile int* const s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
+
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < a.stages; s++) mbar_init(FULL(s), 1), mbar_init(EMPTY(s), 1);
+        for (int p = 0; p < S::kAcc; p++) mbar_init(ACC_FULL(p), 2), mbar_init(ACC_EMPTY(p), S::kEpi);
+        mbar_init(CODES, S::kEpi);
+        mbar_init(SUM_FULL, S::kEpi * split);
+        mbar_init(SUM_FREE, S::kEpi * split);
+        *s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)), "n"(S::kTmem) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    // every CTA of the cluster runs and has its barriers before another one reaches into its shared memory
+    if (split > 1) {
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+    const uint32_t tmem_base = *s_tmem;
+    const int first = blockIdx.x / split, step = gridDim.x / split;
+
+    if (warp == 0) {
+        uint32_t it = 0;
+        bool ok = true;
+        for (int tile = first; tile < a.tiles && ok; tile += step) {
+            const int n0 = tile / a.t_tiles * kRows, t0 = tile % a.t_tiles * NT;
+            for (int kb = kb0; kb < kb1 && ok; kb++, it++) {
+                const int st = it % a.stages;
+                ok = mbar_wait_warp(EMPTY(st), ((it / a.stages) & 1) ^ 1, s_abort, a.err);
+                if (!ok) break;
+                if (elect_one()) {
+                    const uint32_t dst = smem_u32(ring + (size_t)st * S::kStage);
+                    mbar_expect_tx(FULL(st), S::kStage);      // what a box reads past the matrix is zero and counts all the same
+                    tma_load_2d(dst, &tmap_w, kb * kFp8Block, n0, FULL(st));
+                    if (!FUSED) tma_load_2d(dst + kWBytes, &tmap_a, kb * kFp8Block, t0, FULL(st));
+                }
+                __syncwarp();
+            }
+        }
+        // given up: the copies in flight land before the CTA leaves
+        if (!ok)
+            for (uint32_t j = it > (uint32_t)a.stages ? it - a.stages : 0; j < it; j++)
+                for (uint32_t i = 0; i < kSpin && !mbar_try_wait(FULL(j % a.stages), (j / a.stages) & 1); i++) {}
+    } else if (warp == 1) {
+        uint32_t it = 0;
+        bool ok = !FUSED || mbar_wait_warp(CODES, 0, s_abort, a.err);
+        for (int tile = first; tile < a.tiles && ok; tile += step) {
+            for (int i = 0; i < nkb && ok; i++, it++) {
+                const int st = it % a.stages, p = it % S::kAcc;
+                ok = mbar_wait_warp(ACC_EMPTY(p), ((it / S::kAcc) & 1) ^ 1, s_abort, a.err) &&
+                     mbar_wait_warp(FULL(st), (it / a.stages) & 1, s_abort, a.err);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t wsm = smem_u32(ring + (size_t)st * S::kStage);
+                const uint64_t wdesc = umma_desc(wsm), adesc = umma_desc(FUSED ? smem_u32(codes + (size_t)i * S::kABytes) : wsm + kWBytes);
+                if (elect_one()) {
+#pragma unroll
+                    for (int kk = 0; kk < 4; kk++) umma_f8_ss(tmem_base + p * NT, wdesc + kk * 2, adesc + kk * 2, kIdesc, kk > 0);
+                    umma_commit(EMPTY(st));
+                    umma_commit(ACC_FULL(p));
+                }
+                __syncwarp();
+            }
+        }
+    } else if (warp == 2) {
+        // slots of scales, four blocks asked for at a time and the next four before these are handed out
+        constexpr int kPer = (NT + 31) / 32, kAhead = 4;
+        uint32_t it = 0;
+        bool ok = !FUSED || mbar_wait_warp(CODES, 0, s_abort, a.err);
+        float now[kAhead][kPer], next[kAhead][kPer];
+        for (int tile = first; tile < a.tiles && ok; tile += step) {
+            const int nb = tile / a.t_tiles, t0 = tile % a.t_tiles * NT;
+            auto ask = [&](int i0, float (&v)[kAhead][kPer]) {
+#pragma unroll
+                for (int q = 0; q < kAhead; q++) {
+                    const int i = i0 + q;
+                    const float ws = i < nkb ? __ldg(a.w_scale + (size_t)nb * a.blocks + kb0 + i) : 0.f;
+#pragma unroll
+                    for (int j = 0; j < kPer; j++) {
+                        const int col = lane + 32 * j, t = t0 + col;
+                        float s = 0.f;
+                        if (i < nkb && col < NT && t < a.M) s = FUSED ? row_scales[i * NT + col] : a.a_scale[(size_t)(kb0 + i) * a.M + t];
+                        v[q][j] = s * ws;
+                    }
+                }
+            };
+            ask(0, now);
+            for (int i0 = 0; i0 < nkb && ok; i0 += kAhead) {
+                ask(i0 + kAhead, next);
+#pragma unroll
+                for (int q = 0; q < kAhead; q++) {
+                    if (i0 + q >= nkb || !ok) continue;
+                    const int p = it % S::kAcc;
+                    ok = mbar_wait_warp(ACC_EMPTY(p), ((it / S::kAcc) & 1) ^ 1, s_abort, a.err);
+                    if (!ok) continue;
+#pragma unroll
+                    for (int j = 0; j < kPer; j++)
+                        if (lane + 32 * j < NT) slots[p * NT + lane + 32 * j] = now[q][j];
+                    mbar_arrive_warp(ACC_FULL(p));
+                    it++;
+                }
+#pragma unroll
+                for (int q = 0; q < kAhead; q++)
+#pragma unroll
+                    for (int j = 0; j < kPer; j++) now[q][j] = next[q][j];
+            }
+        }
+    } else if (warp >= 4) {
+        const int etid = threadIdx.x - 128, quarter = warp & 3, col0 = (warp - 4) / 4 * S::kCols;
+        if (FUSED) {
+            // sixteen lanes quantise one block of one row, eight elements each, into its place of the swizzled operand
+            for (int w = etid / 16; w < nkb * NT; w += 2 * S::kEpi) {
+                const int i = w / NT, r = w % NT, piece = lane % 16, k = (kb0 + i) * kFp8Block + piece * 8;
+                float f[8];
+                const int valid = r < a.M ? a.K - k : 0;
+                if (a.x_dtype == 0)
+                    fp8_load8(reinterpret_cast<const __nv_bfloat16*>(a.x) + (size_t)r * a.x_stride + k, a.x_vec, valid, f);
+                else
+                    fp8_load8(reinterpret_cast<const float*>(a.x) + (size_t)r * a.x_stride + k, a.x_vec, valid, f);
+                float sc;
+                const uint2 q = fp8_encode8(f, sc);
+                *reinterpret_cast<uint2*>(codes + (size_t)i * S::kABytes + r * 128 + (((piece >> 1) ^ (r & 7)) << 4) + (piece & 1) * 8) = q;
+                if (piece == 0) row_scales[i * NT + r] = sc;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // the tensor core reads these bytes
+            mbar_arrive_warp(CODES);
+        }
+        uint32_t it = 0, done = 0;
+        bool ok = true;
+        const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + col0;
+        for (int tile = first; tile < a.tiles && ok; tile += step, done++) {
+            const int n0 = tile / a.t_tiles * kRows, t0 = tile % a.t_tiles * NT;
+            float acc[S::kCols];
+#pragma unroll
+            for (int j = 0; j < S::kCols; j++) acc[j] = 0.f;
+            for (int i = 0; i < nkb; i++, it++) {
+                const int p = it % S::kAcc;
+                ok = mbar_wait_warp(ACC_FULL(p), (it / S::kAcc) & 1, s_abort, a.err);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                float d[S::kCols / 16][16];
+#pragma unroll
+                for (int q = 0; q < S::kCols / 16; q++) tmem_ld16(taddr + p * NT + q * 16, d[q]);
+                tmem_ld_wait();
+                const float4* const sl = reinterpret_cast<const float4*>(slots + p * NT + col0);
+#pragma unroll
+                for (int q = 0; q < S::kCols / 4; q++) {
+                    const float4 s = sl[q];
+                    const float* const dd = &d[q / 4][q % 4 * 4];
+                    acc[4 * q] = fmaf(dd[0], s.x, acc[4 * q]);
+                    acc[4 * q + 1] = fmaf(dd[1], s.y, acc[4 * q + 1]);
+                    acc[4 * q + 2] = fmaf(dd[2], s.z, acc[4 * q + 2]);
+                    acc[4 * q + 3] = fmaf(dd[3], s.w, acc[4 * q + 3]);
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                mbar_arrive_warp(ACC_EMPTY(p));
+            }
+            if (!ok) break;
+            const int row = quarter * 32 + lane;
+            if (split == 1) {
+                if (n0 + row < a.N) {
+#pragma unroll
+                    for (int j = 0; j < S::kCols; j++)
+                        if (t0 + col0 + j < a.M) store_out(a, t0 + col0 + j, n0 + row, acc[j]);
+                }
+                continue;
+            }
+            // the cluster's sums: token j belongs to the CTA j / share
+            const int share = NT / split;
+            if (done > 0) ok = __all_sync(0xffffffffu, cluster_wait(SUM_FREE, (done - 1) & 1, s_abort, a.err));
+            if (!ok) break;
+#pragma unroll
+            for (int j = 0; j < S::kCols; j++) {
+                const int col = col0 + j;
+                if (t0 + col < a.M) remote_store(map_shared_to(smem_u32(sums + (rank * share + col % share) * kRows + row), col / share), acc[j]);
+            }
+            for (int r = 0; r < split; r++) remote_arrive_warp(map_shared_to(SUM_FULL, r));
+            ok = __all_sync(0xffffffffu, cluster_wait(SUM_FULL, done & 1, s_abort, a.err));
+            if (!ok) break;
+            for (int q = etid; q < share * kRows; q += 32 * S::kEpi) {
+                const int j = q / kRows, n = q % kRows, t = t0 + rank * share + j;
+                if (t < a.M && n0 + n < a.N) {
+                    float v = 0.f;
+                    for (int r = 0; r < split; r++) v += sums[(r * share + j) * kRows + n];
+                    store_out(a, t, n0 + n, v);
+                }
+            }
+            for (int r = 0; r < split; r++) remote_arrive_warp(map_shared_to(SUM_FREE, r));
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "n"(S::kTmem) : "memory");
+    if (split > 1) {      // no CTA leaves while another may still reach into its shared memory
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+}
+
+// codes [rows, K] row-major, box = one block of 128 k by box_rows rows, 128-byte swizzle
+bool make_codes_map(CUtensorMap* map, const void* base, int64_t rows, int64_t K, int box_rows) {
+    EncodeTiledFn fn = encode_tiled();
+    if (!fn) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)K};
+    cuuint32_t box[2] = {(cuuint32_t)kFp8Block, (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+constexpr size_t kSmemLimit = 227 * 1024;
+
+template <int NT, bool FUSED>
+int launch(const uint8_t* codes, const uint8_t* w, Fp8Args a, int sm_count, cudaStream_t s) {
+    using S = Shape<NT, FUSED>;
+    a.blocks = (a.K + kFp8Block - 1) / kFp8Block;
+    a.t_tiles = (a.M + NT - 1) / NT;
+    a.tiles = a.t_tiles * ((a.N + kRows - 1) / kRows);
+    // too few tiles for the SMs: two to eight CTAs share a tile's blocks, two blocks each at least
+    int split = 1;
+    while (split < kMaxSplit && (long long)a.tiles * split * 2 <= sm_count && a.blocks >= split * 4) split *= 2;
+    const int fused_blocks = (a.blocks + split - 1) / split;
+    a.stages = kMaxStages;
+    while (a.stages > 2 && S::bytes(a.stages, split, fused_blocks) > kSmemLimit) a.stages--;
+    const size_t smem = S::bytes(a.stages, split, fused_blocks);
+    CUtensorMap map_w, map_a;
+    if (!make_codes_map(&map_w, w, a.N, a.K, kRows) || (!FUSED && !make_codes_map(&map_a, codes, a.M, a.K, NT))) return -(int)cudaErrorInvalidValue;
+    if (FUSED) map_a = map_w;
+    static PerDeviceOnce once;
+    cudaError_t e = allow_dyn_smem(once, fp8_umma_kernel<NT, FUSED>, kSmemLimit);
+    if (e != cudaSuccess) return -(int)e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(split * max(1, min(a.tiles, sm_count / split)));
+    cfg.blockDim = dim3(S::kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = split;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = split > 1 ? 1 : 0;
+    e = cudaLaunchKernelEx(&cfg, fp8_umma_kernel<NT, FUSED>, map_w, map_a, a, split);
+    return e == cudaSuccess ? 1 : -(int)e;
+}
+
+}  // namespace
+
+// FUSED keeps the codes of sixteen rows in shared memory beside the weight ring
+bool fp8_fused_supported(int M, int K) { return M <= 16 && K <= 8192; }
+
+int launch_fp8_gemm(const uint8_t* a, const float* a_scale, const uint8_t* w, const float* w_scale, int M, int N, int K, void* out,
+                    int out_dtype, long long ldc, int sm_count, int32_t* err, const Ctx& c) {
+    Fp8Args g{};
+    g.a_scale = a_scale; g.w_scale = w_scale; g.M = M; g.N = N; g.K = K; g.c = out; g.c_dtype = out_dtype; g.ldc = ldc; g.err = err;
+    c.begin(K_FP8_GEMM);
+    const int n = M <= 16   ? launch<16, false>(a, w, g, sm_count, c.s)
+                  : M <= 32 ? launch<32, false>(a, w, g, sm_count, c.s)
+                  : M <= 64 ? launch<64, false>(a, w, g, sm_count, c.s)
+                            : launch<128, false>(a, w, g, sm_count, c.s);
+    c.end();
+    return n;
+}
+
+int launch_fp8_linear(const void* x, int x_dtype, long long x_stride, const uint8_t* w, const float* w_scale, int M, int N, int K, void* out,
+                      int out_dtype, long long ldc, int sm_count, int32_t* err, const Ctx& c) {
+    Fp8Args g{};
+    g.x = x; g.x_stride = x_stride; g.x_dtype = x_dtype; g.x_vec = fp8_rows_aligned(x, x_dtype, x_stride);
+    g.w_scale = w_scale; g.M = M; g.N = N; g.K = K; g.c = out; g.c_dtype = out_dtype; g.ldc = ldc; g.err = err;
+    c.begin(K_FP8_GEMM);
+    const int n = launch<16, true>(nullptr, w, g, sm_count, c.s);
+    c.end();
+    return n;
+}
+
+}  // namespace ftm

@@ -256,10 +256,15 @@ bool dense_gemv_supported(int N, int K);
 int launch_dense_gemv(const void* a, int a_dtype, const uint32_t* packed, const uint8_t* scale, const uint16_t* global,
                       int M, int N, int K, float* c, int sm_count, int32_t* err, const Ctx& ctx);
 
-// fp8.cu: block-scaled 8-bit products and the quantisation of their activations
+// fp8_quantize.cu, fp8_umma.cu: block-scaled 8-bit products and the quantisation of their activations; a negative result is a
+// CUDA error code
 int launch_fp8_quantize(const void* x, int x_dtype, int rows, int K, long long stride, uint8_t* q, float* scale, const Ctx& c);
 int launch_fp8_gemm(const uint8_t* a, const float* a_scale, const uint8_t* w, const float* w_scale, int M, int N, int K, void* out,
-                    int out_dtype, long long ldc, const Ctx& c);
+                    int out_dtype, long long ldc, int sm_count, int32_t* err, const Ctx& c);
+// quantisation and product in one kernel
+bool fp8_fused_supported(int M, int K);
+int launch_fp8_linear(const void* x, int x_dtype, long long x_stride, const uint8_t* w, const float* w_scale, int M, int N, int K, void* out,
+                      int out_dtype, long long ldc, int sm_count, int32_t* err, const Ctx& c);
 
 // logprobs.cu: what a server reads off its logits; a negative result is a CUDA error code
 int launch_logprobs(const void* logits, int dtype, int rows, int vocab, long long stride, const void* ids, int ids_dtype, int top_n,

@@ -272,8 +272,9 @@ FTM_API int ftm_fp8_quantize(ftm_handle* h, const void* x, int x_dtype, int32_t 
  * m and n.  The same inputs give the same bits.  Asynchronous. */
 FTM_API int ftm_fp8_gemm(ftm_handle* h, const void* a_e4m3, const float* a_scale, const void* w_e4m3, const float* w_scale, int32_t m,
                          int32_t n, int32_t k, void* c, int c_dtype, int64_t c_stride, void* stream);
-/* ftm_fp8_gemm of ftm_fp8_quantize(x) in one call.  q_scratch [m, k] (16-byte aligned) and scale_scratch
- * [ceil(k / 128), m] f32 are the caller's, so calls that overlap on the GPU do not meet in them.  Asynchronous. */
+/* ftm_fp8_gemm of ftm_fp8_quantize(x) in one call; for up to 16 rows of up to 8192 elements in one kernel, which needs no scratch
+ * (both may be NULL).  Above that q_scratch [m, k] (16-byte aligned) and scale_scratch [ceil(k / 128), m] f32 are the caller's,
+ * so calls that overlap on the GPU do not meet in them.  Asynchronous. */
 FTM_API int ftm_fp8_linear(ftm_handle* h, const void* x, int x_dtype, int64_t x_stride, const void* w_e4m3, const float* w_scale,
                            int32_t m, int32_t n, int32_t k, void* q_scratch, float* scale_scratch, void* c, int c_dtype,
                            int64_t c_stride, void* stream);
