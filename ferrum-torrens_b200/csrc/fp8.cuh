@@ -36,22 +36,35 @@ __device__ __forceinline__ void fp8_load8(const T* p, bool vec, int valid, float
     }
 }
 
-// The codes of this lane's eight elements of a block that sixteen neighbouring lanes hold, and the block's scale.  Rounds to
-// nearest even, saturates; a NaN stays one and does not count as a magnitude.
-__device__ __forceinline__ uint2 fp8_encode8(const float (&f)[8], float& scale) {
-    float most = 0.f;
+// Codes and scales of U blocks at once, each held by sixteen neighbouring lanes, eight elements per lane.  Rounds to nearest even,
+// saturates; a NaN stays one and does not count as a magnitude.  The 2 U quotients of a group are one division, of lane j < 2 U.
+template <int U>
+__device__ __forceinline__ void fp8_encode(const float (&f)[U][8], uint2 (&codes)[U], float (&scale)[U]) {
+    static_assert(U <= 8, "a lane for each quotient");
+    const int lane = threadIdx.x % 16, group = threadIdx.x % 32 - lane;
+    float num = 1.f, den = 1.f;
 #pragma unroll
-    for (int j = 0; j < 8; j++) most = fmaxf(most, fabsf(f[j]));
+    for (int u = 0; u < U; u++) {
+        float most = 0.f;
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    most = fmaxf(most, kFp8Least);
-    const float inv = __fdiv_rn(kFp8Max, most);
-    scale = __fdiv_rn(most, kFp8Max);
-    uint32_t c[4];
+        for (int j = 0; j < 8; j++) most = fmaxf(most, fabsf(f[u][j]));
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-        c[j] = __nv_cvt_float2_to_fp8x2(make_float2(f[2 * j] * inv, f[2 * j + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-    return make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+        for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        most = fmaxf(most, kFp8Least);
+        if (lane == 2 * u) num = kFp8Max, den = most;
+        if (lane == 2 * u + 1) num = most, den = kFp8Max;
+    }
+    const float quotient = __fdiv_rn(num, den);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const float inv = __shfl_sync(0xffffffffu, quotient, group + 2 * u);
+        scale[u] = __shfl_sync(0xffffffffu, quotient, group + 2 * u + 1);
+        uint32_t c[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            c[j] = __nv_cvt_float2_to_fp8x2(make_float2(f[u][2 * j] * inv, f[u][2 * j + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+        codes[u] = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+    }
 }
 
 inline bool fp8_rows_aligned(const void* x, int x_dtype, long long stride) {

@@ -10,19 +10,29 @@ namespace ftm {
 
 namespace {
 
+constexpr int kAtOnce = 2;      // blocks a group of lanes holds at a time
+
 template <typename T>
 __global__ void __launch_bounds__(256)
 fp8_quantize_kernel(const T* __restrict__ x, long long stride, int rows, int K, bool vec, uint8_t* __restrict__ q, float* __restrict__ scale) {
     const int lane = threadIdx.x % 32, blocks = (K + kFp8Block - 1) / kFp8Block;
     const long long row = (long long)blockIdx.x * 8 + threadIdx.x / 32;
     if (row >= rows) return;
-    for (int b = blockIdx.y * 2 + lane / 16; b - lane / 16 < blocks; b += gridDim.y * 2) {
-        const int k = b * kFp8Block + (lane % 16) * 8;
-        float f[8], sc;
-        fp8_load8(x + row * stride + k, vec, b < blocks ? K - k : 0, f);
-        const uint2 codes = fp8_encode8(f, sc);
-        if (b < blocks && k < K) *reinterpret_cast<uint2*>(q + row * K + k) = codes;
-        if (b < blocks && lane % 16 == 0) scale[(long long)b * rows + row] = sc;
+    for (int b0 = blockIdx.y * 2 * kAtOnce; b0 < blocks; b0 += gridDim.y * 2 * kAtOnce) {
+        float f[kAtOnce][8], sc[kAtOnce];
+        uint2 codes[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; u++) {
+            const int b = b0 + 2 * u + lane / 16, k = b * kFp8Block + (lane % 16) * 8;
+            fp8_load8(x + row * stride + k, vec, b < blocks ? K - k : 0, f[u]);
+        }
+        fp8_encode(f, codes, sc);
+#pragma unroll
+        for (int u = 0; u < kAtOnce; u++) {
+            const int b = b0 + 2 * u + lane / 16, k = b * kFp8Block + (lane % 16) * 8;
+            if (b < blocks && k < K) *reinterpret_cast<uint2*>(q + row * K + k) = codes[u];
+            if (b < blocks && lane % 16 == 0) scale[(long long)b * rows + row] = sc[u];
+        }
     }
 }
 
@@ -31,7 +41,7 @@ fp8_quantize_kernel(const T* __restrict__ x, long long stride, int rows, int K, 
 int launch_fp8_quantize(const void* x, int x_dtype, int rows, int K, long long stride, uint8_t* q, float* scale, const Ctx& c) {
     const int blocks = (K + kFp8Block - 1) / kFp8Block;
     const bool vec = fp8_rows_aligned(x, x_dtype, stride);
-    const dim3 grid(((unsigned)rows + 7) / 8, min((blocks + 1) / 2, 65535));
+    const dim3 grid(((unsigned)rows + 7) / 8, min((blocks + 2 * kAtOnce - 1) / (2 * kAtOnce), 65535));
     c.begin(K_FP8_QUANTIZE);
     if (x_dtype == 0)
         fp8_quantize_kernel<<<grid, 256, 0, c.s>>>((const __nv_bfloat16*)x, stride, rows, K, vec, q, scale);

@@ -51,15 +51,15 @@ __device__ __forceinline__ uint32_t map_shared_to(uint32_t addr, uint32_t rank) 
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
-__device__ __forceinline__ void remote_store(uint32_t addr, float v) {
-    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+// a store into another CTA's shared memory that counts its bytes on a barrier there: no fence, and who waits sees the value
+__device__ __forceinline__ void remote_store(uint32_t addr, float v, uint32_t bar) {
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(addr), "r"(__float_as_uint(v)), "r"(bar) : "memory");
 }
-// one arrival of a converged warp on a barrier of another CTA; what its lanes stored before is visible to who waits there
-__device__ __forceinline__ void remote_arrive_warp(uint32_t bar) {
-    asm volatile("fence.acq_rel.cluster;" ::: "memory");
-    __syncwarp();
-    if (threadIdx.x % 32 == 0) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+__device__ __forceinline__ void remote_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_join() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ bool cluster_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* err) {
     for (uint32_t i = 0; i < kSpin; i++) {
         uint32_t ok;
@@ -77,6 +77,16 @@ __device__ __forceinline__ bool cluster_wait(uint32_t bar, uint32_t parity, vola
     atomicExch(err, 3);
     return false;
 }
+
+// a place in a ring of n and the parity of the round
+struct Ring {
+    int n, i = 0;
+    uint32_t round = 0;
+    __device__ __forceinline__ explicit Ring(int size) : n(size) {}
+    __device__ __forceinline__ void next() {
+        if (++i == n) i = 0, round ^= 1;
+    }
+};
 
 struct Fp8Args {
     const void* x;               // FUSED: the rows
@@ -96,7 +106,8 @@ struct Fp8Args {
 template <int NT, bool FUSED>
 struct Shape {
     static constexpr int kEpi = NT >= 64 ? 8 : 4;                // epilogue warps
-    static constexpr int kThreads = 128 + 32 * kEpi;
+    static constexpr int kHelp = FUSED ? 4 : 0;                  // more warps that quantise
+    static constexpr int kThreads = 128 + 32 * (kEpi + kHelp);
     static constexpr int kCols = NT * 4 / kEpi;                  // columns of one epilogue warp
     static constexpr int kAcc = NT >= 128 ? 2 : 4;               // accumulators (and slots of scales)
     static constexpr int kTmem = NT * kAcc < 32 ? 32 : NT * kAcc;
@@ -108,8 +119,6 @@ struct Shape {
                kAcc * NT * 4 + kBarBytes;
     }
 };
-
-__device__ __forceinline__ void store_out(const Fp8Args& a, int t, int n, float v) { store_act(a.c, a.c_dtype, (size_t)t * a.ldc + n, v); }
 
 template <int NT, bool FUSED>
 __global__ void __launch_bounds__(Shape<NT, FUSED>::kThreads, 1)
@@ -136,13 +145,15 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     volatile int* const s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < a.stages; s++) mbar_init(FULL(s), 1), mbar_init(EMPTY(s), 1);
-        for (int p = 0; p < S::kAcc; p++) mbar_init(ACC_FULL(p), 2), mbar_init(ACC_EMPTY(p), S::kEpi);
-        mbar_init(CODES, S::kEpi);
-        mbar_init(SUM_FULL, S::kEpi * split);
-        mbar_init(SUM_FREE, S::kEpi * split);
-        *s_abort = 0;
+    if (warp == 0) {
+        if (lane < a.stages) mbar_init(FULL(lane), 1), mbar_init(EMPTY(lane), 1);
+        if (lane < S::kAcc) mbar_init(ACC_FULL(lane), 2), mbar_init(ACC_EMPTY(lane), S::kEpi);
+        if (lane == 0) {
+            mbar_init(CODES, S::kEpi + S::kHelp);
+            mbar_init(SUM_FULL, 1);
+            mbar_init(SUM_FREE, S::kEpi * split);
+            *s_abort = 0;
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 2) {
@@ -152,61 +163,64 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    // every CTA of the cluster runs and has its barriers before another one reaches into its shared memory
-    if (split > 1) {
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    }
+    // Two barriers of the cluster.  The first: every CTA runs and has its barriers before another one reaches into its shared
+    // memory (waited for before the first sums are sent).  The second: none leaves while another may still reach into it.
+    if (split > 1) cluster_arrive();
     const uint32_t tmem_base = *s_tmem;
     const int first = blockIdx.x / split, step = gridDim.x / split;
+    bool joined = split == 1, left = split == 1;      // this thread has waited for the first, has arrived at the second
 
     if (warp == 0) {
-        uint32_t it = 0;
+        Ring st(a.stages);
         bool ok = true;
+        uint32_t asked = 0;
         for (int tile = first; tile < a.tiles && ok; tile += step) {
             const int n0 = tile / a.t_tiles * kRows, t0 = tile % a.t_tiles * NT;
-            for (int kb = kb0; kb < kb1 && ok; kb++, it++) {
-                const int st = it % a.stages;
-                ok = mbar_wait_warp(EMPTY(st), ((it / a.stages) & 1) ^ 1, s_abort, a.err);
+            for (int kb = kb0; kb < kb1; kb++, st.next(), asked++) {
+                ok = mbar_wait_warp(EMPTY(st.i), st.round ^ 1, s_abort, a.err);
                 if (!ok) break;
                 if (elect_one()) {
-                    const uint32_t dst = smem_u32(ring + (size_t)st * S::kStage);
-                    mbar_expect_tx(FULL(st), S::kStage);      // what a box reads past the matrix is zero and counts all the same
-                    tma_load_2d(dst, &tmap_w, kb * kFp8Block, n0, FULL(st));
-                    if (!FUSED) tma_load_2d(dst + kWBytes, &tmap_a, kb * kFp8Block, t0, FULL(st));
+                    const uint32_t dst = smem_u32(ring + st.i * S::kStage);
+                    mbar_expect_tx(FULL(st.i), S::kStage);      // what a box reads past the matrix is zero and counts all the same
+                    tma_load_2d(dst, &tmap_w, kb * kFp8Block, n0, FULL(st.i));
+                    if (!FUSED) tma_load_2d(dst + kWBytes, &tmap_a, kb * kFp8Block, t0, FULL(st.i));
                 }
                 __syncwarp();
             }
         }
         // given up: the copies in flight land before the CTA leaves
         if (!ok)
-            for (uint32_t j = it > (uint32_t)a.stages ? it - a.stages : 0; j < it; j++)
+            for (uint32_t j = asked > (uint32_t)a.stages ? asked - a.stages : 0; j < asked; j++)
                 for (uint32_t i = 0; i < kSpin && !mbar_try_wait(FULL(j % a.stages), (j / a.stages) & 1); i++) {}
     } else if (warp == 1) {
-        uint32_t it = 0;
-        bool ok = !FUSED || mbar_wait_warp(CODES, 0, s_abort, a.err);
+        Ring st(a.stages), p(S::kAcc);
+        bool ok = !FUSED || mbar_wait_warp(CODES, 0, s_abort, a.err), seen = false;
         for (int tile = first; tile < a.tiles && ok; tile += step) {
-            for (int i = 0; i < nkb && ok; i++, it++) {
-                const int st = it % a.stages, p = it % S::kAcc;
-                ok = mbar_wait_warp(ACC_EMPTY(p), ((it / S::kAcc) & 1) ^ 1, s_abort, a.err) &&
-                     mbar_wait_warp(FULL(st), (it / a.stages) & 1, s_abort, a.err);
-                if (!ok) break;
+            for (int i = 0; i < nkb; i++) {
+                if (!seen) {
+                    ok = mbar_wait_warp(ACC_EMPTY(p.i), p.round ^ 1, s_abort, a.err) && mbar_wait_warp(FULL(st.i), st.round, s_abort, a.err);
+                    if (!ok) break;
+                }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t wsm = smem_u32(ring + (size_t)st * S::kStage);
-                const uint64_t wdesc = umma_desc(wsm), adesc = umma_desc(FUSED ? smem_u32(codes + (size_t)i * S::kABytes) : wsm + kWBytes);
+                const uint32_t wsm = smem_u32(ring + st.i * S::kStage);
+                const uint64_t wdesc = umma_desc(wsm), adesc = umma_desc(FUSED ? smem_u32(codes + i * S::kABytes) : wsm + kWBytes);
                 if (elect_one()) {
 #pragma unroll
-                    for (int kk = 0; kk < 4; kk++) umma_f8_ss(tmem_base + p * NT, wdesc + kk * 2, adesc + kk * 2, kIdesc, kk > 0);
-                    umma_commit(EMPTY(st));
-                    umma_commit(ACC_FULL(p));
+                    for (int kk = 0; kk < 4; kk++) umma_f8_ss(tmem_base + p.i * NT, wdesc + kk * 2, adesc + kk * 2, kIdesc, kk > 0);
+                    umma_commit(EMPTY(st.i));
+                    umma_commit(ACC_FULL(p.i));
                 }
                 __syncwarp();
+                st.next();
+                p.next();
+                // a look at the next block's barriers while these products run
+                seen = __all_sync(0xffffffffu, mbar_test_wait(ACC_EMPTY(p.i), p.round ^ 1) & mbar_test_wait(FULL(st.i), st.round));
             }
         }
     } else if (warp == 2) {
         // slots of scales, four blocks asked for at a time and the next four before these are handed out
         constexpr int kPer = (NT + 31) / 32, kAhead = 4;
-        uint32_t it = 0;
+        Ring p(S::kAcc);
         bool ok = !FUSED || mbar_wait_warp(CODES, 0, s_abort, a.err);
         float now[kAhead][kPer], next[kAhead][kPer];
         for (int tile = first; tile < a.tiles && ok; tile += step) {
@@ -231,14 +245,13 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
 #pragma unroll
                 for (int q = 0; q < kAhead; q++) {
                     if (i0 + q >= nkb || !ok) continue;
-                    const int p = it % S::kAcc;
-                    ok = mbar_wait_warp(ACC_EMPTY(p), ((it / S::kAcc) & 1) ^ 1, s_abort, a.err);
+                    ok = mbar_wait_warp(ACC_EMPTY(p.i), p.round ^ 1, s_abort, a.err);
                     if (!ok) continue;
 #pragma unroll
                     for (int j = 0; j < kPer; j++)
-                        if (lane + 32 * j < NT) slots[p * NT + lane + 32 * j] = now[q][j];
-                    mbar_arrive_warp(ACC_FULL(p));
-                    it++;
+                        if (lane + 32 * j < NT) slots[p.i * NT + lane + 32 * j] = now[q][j];
+                    mbar_arrive_warp(ACC_FULL(p.i));
+                    p.next();
                 }
 #pragma unroll
                 for (int q = 0; q < kAhead; q++)
@@ -249,41 +262,58 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     } else if (warp >= 4) {
         const int etid = threadIdx.x - 128, quarter = warp & 3, col0 = (warp - 4) / 4 * S::kCols;
         if (FUSED) {
-            // sixteen lanes quantise one block of one row, eight elements each, into its place of the swizzled operand
-            for (int w = etid / 16; w < nkb * NT; w += 2 * S::kEpi) {
-                const int i = w / NT, r = w % NT, piece = lane % 16, k = (kb0 + i) * kFp8Block + piece * 8;
-                float f[8];
-                const int valid = r < a.M ? a.K - k : 0;
-                if (a.x_dtype == 0)
-                    fp8_load8(reinterpret_cast<const __nv_bfloat16*>(a.x) + (size_t)r * a.x_stride + k, a.x_vec, valid, f);
-                else
-                    fp8_load8(reinterpret_cast<const float*>(a.x) + (size_t)r * a.x_stride + k, a.x_vec, valid, f);
-                float sc;
-                const uint2 q = fp8_encode8(f, sc);
-                *reinterpret_cast<uint2*>(codes + (size_t)i * S::kABytes + r * 128 + (((piece >> 1) ^ (r & 7)) << 4) + (piece & 1) * 8) = q;
-                if (piece == 0) row_scales[i * NT + r] = sc;
+            // rows past M are zero
+            for (int w = etid; w < nkb * (NT * 8); w += 32 * (S::kEpi + S::kHelp))
+                if (w / 8 % NT >= a.M) *reinterpret_cast<uint4*>(codes + w * 16) = make_uint4(0, 0, 0, 0);
+            // sixteen lanes quantise one block of one row, eight elements each, into its place of the swizzled operand; all of a
+            // pass's rows are asked for before the first is used
+            constexpr int kGroups = 2 * (S::kEpi + S::kHelp), kAtOnce = 4;
+            const int piece = lane % 16, units = nkb * a.M;
+            const uint32_t by_m = 65536u / a.M + 1;      // (w * by_m) >> 16 = w / M for w < 65536 / M
+            for (int w0 = etid / 32 * 2; w0 < units; w0 += kGroups * kAtOnce) {
+                float f[kAtOnce][8], sc[kAtOnce];
+                uint2 q[kAtOnce];
+                int at[kAtOnce], row[kAtOnce];
+#pragma unroll
+                for (int u = 0; u < kAtOnce; u++) {
+                    const int w = w0 + lane / 16 + u * kGroups, i = (w * by_m) >> 16, r = w - i * a.M, k = (kb0 + i) * kFp8Block + piece * 8;
+                    const int valid = w < units ? a.K - k : 0;
+                    at[u] = i, row[u] = r;
+                    if (a.x_dtype == 0)
+                        fp8_load8(reinterpret_cast<const __nv_bfloat16*>(a.x) + r * a.x_stride + k, a.x_vec, valid, f[u]);
+                    else
+                        fp8_load8(reinterpret_cast<const float*>(a.x) + r * a.x_stride + k, a.x_vec, valid, f[u]);
+                }
+                fp8_encode(f, q, sc);
+#pragma unroll
+                for (int u = 0; u < kAtOnce; u++) {
+                    if (w0 + lane / 16 + u * kGroups >= units) continue;
+                    *reinterpret_cast<uint2*>(codes + at[u] * S::kABytes + row[u] * 128 + (((piece >> 1) ^ (row[u] & 7)) << 4) + (piece & 1) * 8) = q[u];
+                    if (piece == 0) row_scales[at[u] * NT + row[u]] = sc[u];
+                }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // the tensor core reads these bytes
             mbar_arrive_warp(CODES);
         }
-        uint32_t it = 0, done = 0;
+        Ring p(S::kAcc);
+        uint32_t done = 0, got = 0;
         bool ok = true;
         const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + col0;
-        for (int tile = first; tile < a.tiles && ok; tile += step, done++) {
+        const int row = quarter * 32 + lane;
+        for (int tile = first; tile < a.tiles && ok && warp < 4 + S::kEpi; tile += step, done++) {
             const int n0 = tile / a.t_tiles * kRows, t0 = tile % a.t_tiles * NT;
             float acc[S::kCols];
 #pragma unroll
             for (int j = 0; j < S::kCols; j++) acc[j] = 0.f;
-            for (int i = 0; i < nkb; i++, it++) {
-                const int p = it % S::kAcc;
-                ok = mbar_wait_warp(ACC_FULL(p), (it / S::kAcc) & 1, s_abort, a.err);
+            for (int i = 0; i < nkb; i++, p.next()) {
+                ok = mbar_wait_warp(ACC_FULL(p.i), p.round, s_abort, a.err);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 float d[S::kCols / 16][16];
 #pragma unroll
-                for (int q = 0; q < S::kCols / 16; q++) tmem_ld16(taddr + p * NT + q * 16, d[q]);
+                for (int q = 0; q < S::kCols / 16; q++) tmem_ld16(taddr + p.i * NT + q * 16, d[q]);
                 tmem_ld_wait();
-                const float4* const sl = reinterpret_cast<const float4*>(slots + p * NT + col0);
+                const float4* const sl = reinterpret_cast<const float4*>(slots + p.i * NT + col0);
 #pragma unroll
                 for (int q = 0; q < S::kCols / 4; q++) {
                     const float4 s = sl[q];
@@ -294,48 +324,65 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
                     acc[4 * q + 3] = fmaf(dd[3], s.w, acc[4 * q + 3]);
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                mbar_arrive_warp(ACC_EMPTY(p));
+                mbar_arrive_warp(ACC_EMPTY(p.i));
             }
             if (!ok) break;
-            const int row = quarter * 32 + lane;
             if (split == 1) {
-                if (n0 + row < a.N) {
+                // a warp's lanes are neighbouring weight rows: one store is 64 or 128 contiguous bytes of a token's output
+                const int cols = n0 + row < a.N ? min(S::kCols, a.M - t0 - col0) : 0;
+                const long long base = (long long)(t0 + col0) * a.ldc + n0 + row;
+                if (a.c_dtype == 0) {
+                    __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(a.c) + base;
 #pragma unroll
-                    for (int j = 0; j < S::kCols; j++)
-                        if (t0 + col0 + j < a.M) store_out(a, t0 + col0 + j, n0 + row, acc[j]);
+                    for (int j = 0; j < S::kCols; j++, o += a.ldc)
+                        if (j < cols) *o = __float2bfloat16_rn(acc[j]);
+                } else {
+                    float* o = reinterpret_cast<float*>(a.c) + base;
+#pragma unroll
+                    for (int j = 0; j < S::kCols; j++, o += a.ldc)
+                        if (j < cols) *o = acc[j];
                 }
                 continue;
             }
-            // the cluster's sums: token j belongs to the CTA j / share
-            const int share = NT / split;
+            // the cluster's sums: token j belongs to the CTA j / share (a power of two)
+            const int log_share = __ffs(NT / split) - 1, share = NT / split, mine = min(share, a.M - t0 - rank * share);
+            const bool last = tile + step >= a.tiles;
+            if (etid == 0 && mine > 0) mbar_expect_tx(SUM_FULL, split * mine * kRows * 4);
+            if (!joined) cluster_join(), joined = true;
             if (done > 0) ok = __all_sync(0xffffffffu, cluster_wait(SUM_FREE, (done - 1) & 1, s_abort, a.err));
             if (!ok) break;
+            const uint32_t to_sums = smem_u32(sums + rank * share * kRows + row);
 #pragma unroll
             for (int j = 0; j < S::kCols; j++) {
-                const int col = col0 + j;
-                if (t0 + col < a.M) remote_store(map_shared_to(smem_u32(sums + (rank * share + col % share) * kRows + row), col / share), acc[j]);
+                const int col = col0 + j, to = col >> log_share;
+                if (t0 + col < a.M)
+                    remote_store(map_shared_to(to_sums + (col & (share - 1)) * kRows * 4, to), acc[j], map_shared_to(SUM_FULL, to));
             }
-            for (int r = 0; r < split; r++) remote_arrive_warp(map_shared_to(SUM_FULL, r));
-            ok = __all_sync(0xffffffffu, cluster_wait(SUM_FULL, done & 1, s_abort, a.err));
-            if (!ok) break;
-            for (int q = etid; q < share * kRows; q += 32 * S::kEpi) {
-                const int j = q / kRows, n = q % kRows, t = t0 + rank * share + j;
-                if (t < a.M && n0 + n < a.N) {
-                    float v = 0.f;
-                    for (int r = 0; r < split; r++) v += sums[(r * share + j) * kRows + n];
-                    store_out(a, t, n0 + n, v);
+            __syncwarp();
+            if (last) cluster_arrive(), left = true;      // nothing of this warp's goes to another CTA from here on
+            if (mine > 0) {
+                ok = __all_sync(0xffffffffu, cluster_wait(SUM_FULL, got++ & 1, s_abort, a.err));
+                if (!ok) break;
+                for (int q = etid; q < mine * kRows; q += 32 * S::kEpi) {
+                    const int j = q / kRows, n = q % kRows;
+                    float v[kMaxSplit], sum = 0.f;
+#pragma unroll
+                    for (int r = 0; r < kMaxSplit; r++) v[r] = r < split ? sums[(r * share + j) * kRows + n] : 0.f;
+#pragma unroll
+                    for (int r = 0; r < kMaxSplit; r++) sum += v[r];
+                    if (n0 + n < a.N) store_act(a.c, a.c_dtype, (size_t)(t0 + rank * share + j) * a.ldc + n0 + n, sum);
                 }
             }
-            for (int r = 0; r < split; r++) remote_arrive_warp(map_shared_to(SUM_FREE, r));
+            __syncwarp();
+            if (!last && lane < split) remote_arrive(map_shared_to(SUM_FREE, lane));
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "n"(S::kTmem) : "memory");
-    if (split > 1) {      // no CTA leaves while another may still reach into its shared memory
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    }
+    if (!joined) cluster_join();
+    if (!left) cluster_arrive();
+    if (split > 1) cluster_join();
 }
 
 // codes [rows, K] row-major, box = one block of 128 k by box_rows rows, 128-byte swizzle
