@@ -8,7 +8,7 @@
 // block, so a sum over all of k cannot stay in tensor memory; with two or four accumulators the next blocks are
 // multiplied meanwhile.
 //   warp 0      TMA: weight box [128 rows x 128 k], token box [NT x 128 k]
-//   warp 1      issues the products
+//   warps 1, 3  issue the products, a block each in turn
 //   warp 2      allocates the tensor memory; multiplies the two scales of every (block, token) ahead of the epilogue
 //   warps 4..   epilogue: four warps for NT <= 32, eight above (each four take half of the columns)
 // Few tiles: the blocks of k are split over the CTAs of a cluster.  Every CTA stores its sums of the tokens that CTA r finishes into r's
@@ -58,8 +58,8 @@ __device__ __forceinline__ void remote_store(uint32_t addr, float v, uint32_t ba
 __device__ __forceinline__ void remote_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_join() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_join() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 __device__ __forceinline__ bool cluster_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* err) {
     for (uint32_t i = 0; i < kSpin; i++) {
         uint32_t ok;
@@ -112,16 +112,19 @@ struct Shape {
     static constexpr int kAcc = NT >= 128 ? 2 : 4;               // accumulators (and slots of scales)
     static constexpr int kTmem = NT * kAcc < 32 ? 32 : NT * kAcc;
     static constexpr int kABytes = NT * kFp8Block;               // a token box
+    static constexpr int kPerSm = NT <= 32 ? 2 : 1;              // CTAs of an SM
+    static constexpr size_t kSmem = kPerSm == 2 ? 113 * 1024 : 227 * 1024;
     static constexpr int kStage = kWBytes + (FUSED ? 0 : kABytes);
     // after the ring: sums from the cluster's CTAs [ranks][NT / ranks][128], slots of scales, FUSED: codes and scales of the rows
+    static __host__ __device__ int sum_floats(int split) { return (NT + split - 1) / split * split * kRows; }
     static size_t bytes(int stages, int split, int fused_blocks) {
-        return 1024 + (size_t)stages * kStage + (FUSED ? (size_t)fused_blocks * (kABytes + NT * 4) : 0) + (split > 1 ? (size_t)NT * kRows * 4 : 0) +
+        return 1024 + (size_t)stages * kStage + (FUSED ? (size_t)fused_blocks * (kABytes + NT * 4) : 0) + (split > 1 ? (size_t)sum_floats(split) * 4 : 0) +
                kAcc * NT * 4 + kBarBytes;
     }
 };
 
 template <int NT, bool FUSED>
-__global__ void __launch_bounds__(Shape<NT, FUSED>::kThreads, 1)
+__global__ void __launch_bounds__(Shape<NT, FUSED>::kThreads, (Shape<NT, FUSED>::kPerSm))
 fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_a, const Fp8Args a, const int split) {
     using S = Shape<NT, FUSED>;
     constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(NT >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);   // e4m3 x e4m3 -> f32
@@ -132,7 +135,7 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     const int max_nkb = (a.blocks + split - 1) / split;
     uint8_t* const codes = ring + (size_t)a.stages * S::kStage;                          // FUSED [max_nkb][NT x 128]
     float* const sums = reinterpret_cast<float*>(codes + (FUSED ? (size_t)max_nkb * S::kABytes : 0));
-    float* const slots = sums + (split > 1 ? NT * kRows : 0);                            // [kAcc][NT]
+    float* const slots = sums + (split > 1 ? S::sum_floats(split) : 0);                            // [kAcc][NT]
     float* const row_scales = slots + S::kAcc * NT;                                      // FUSED [max_nkb][NT]
     uint64_t* const bars = reinterpret_cast<uint64_t*>(row_scales + (FUSED ? max_nkb * NT : 0));
     const uint32_t bar0 = smem_u32(bars);
@@ -140,25 +143,70 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     auto EMPTY = [&](int s) { return bar0 + 8u * (kMaxStages + s); };
     auto ACC_FULL = [&](int p) { return bar0 + 8u * (2 * kMaxStages + p); };
     auto ACC_EMPTY = [&](int p) { return bar0 + 8u * (2 * kMaxStages + kMaxAcc + p); };
-    const uint32_t CODES = bar0 + 8u * (2 * kMaxStages + 2 * kMaxAcc), SUM_FULL = CODES + 8, SUM_FREE = CODES + 16;
+    const uint32_t SUM_FULL = bar0 + 8u * (2 * kMaxStages + 2 * kMaxAcc), SUM_FREE = SUM_FULL + 8;
     uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(bars + 2 * kMaxStages + 2 * kMaxAcc + 4);
     volatile int* const s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int first = blockIdx.x / split, step = gridDim.x / split;
+    auto load = [&](int st, int tile, int kb) {
+        const uint32_t dst = smem_u32(ring + st * S::kStage);
+        mbar_expect_tx(FULL(st), S::kStage);      // what a box reads past the matrix is zero and counts all the same
+        tma_load_2d(dst, &tmap_w, kb * kFp8Block, tile / a.t_tiles * kRows, FULL(st));
+        if (!FUSED) tma_load_2d(dst + kWBytes, &tmap_a, kb * kFp8Block, tile % a.t_tiles * NT, FULL(st));
+    };
+    const int early = min(2, nkb);         // blocks of the first tile that are asked for before the CTA is set up
     if (warp == 0) {
         if (lane < a.stages) mbar_init(FULL(lane), 1), mbar_init(EMPTY(lane), 1);
         if (lane < S::kAcc) mbar_init(ACC_FULL(lane), 2), mbar_init(ACC_EMPTY(lane), S::kEpi);
         if (lane == 0) {
-            mbar_init(CODES, S::kEpi + S::kHelp);
             mbar_init(SUM_FULL, 1);
             mbar_init(SUM_FREE, S::kEpi * split);
             *s_abort = 0;
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        __syncwarp();
+        if (elect_one())
+            for (int i = 0; i < early; i++) load(i, first, kb0 + i);
+        __syncwarp();
     }
     if (warp == 2) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)), "n"(S::kTmem) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (FUSED && warp >= 4) {
+        const int etid = threadIdx.x - 128;
+        // sixteen lanes quantise one block of one row, eight elements each, into its place of the swizzled operand; all of a
+        // pass's rows are asked for before the first is used
+        constexpr int kGroups = 2 * (S::kEpi + S::kHelp), kAtOnce = 4;
+        const int piece = lane % 16, units = nkb * a.M;
+        const uint32_t by_m = 65536u / a.M + 1;      // (w * by_m) >> 16 = w / M for w < 65536 / M
+        for (int w0 = etid / 32 * 2; w0 < units; w0 += kGroups * kAtOnce) {
+            float f[kAtOnce][8], sc[kAtOnce];
+            uint2 q[kAtOnce];
+            int at[kAtOnce], row[kAtOnce];
+#pragma unroll
+            for (int u = 0; u < kAtOnce; u++) {
+                const int w = w0 + lane / 16 + u * kGroups, i = (w * by_m) >> 16, r = w - i * a.M, k = (kb0 + i) * kFp8Block + piece * 8;
+                const int valid = w < units ? a.K - k : 0;
+                at[u] = i, row[u] = r;
+                if (a.x_dtype == 0)
+                    fp8_load8(reinterpret_cast<const __nv_bfloat16*>(a.x) + r * a.x_stride + k, a.x_vec, valid, f[u]);
+                else
+                    fp8_load8(reinterpret_cast<const float*>(a.x) + r * a.x_stride + k, a.x_vec, valid, f[u]);
+            }
+            fp8_encode(f, q, sc);
+#pragma unroll
+            for (int u = 0; u < kAtOnce; u++) {
+                if (w0 + lane / 16 + u * kGroups >= units) continue;
+                *reinterpret_cast<uint2*>(codes + at[u] * S::kABytes + row[u] * 128 + (((piece >> 1) ^ (row[u] & 7)) << 4) + (piece & 1) * 8) = q[u];
+                if (piece == 0) row_scales[at[u] * NT + row[u]] = sc[u];
+            }
+        }
+        // rows past M are zero
+        for (int w = etid; w < nkb * (NT * 8); w += 32 * (S::kEpi + S::kHelp))
+            if (w / 8 % NT >= a.M) *reinterpret_cast<uint4*>(codes + w * 16) = make_uint4(0, 0, 0, 0);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // the tensor core reads these bytes
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -167,7 +215,6 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     // memory (waited for before the first sums are sent).  The second: none leaves while another may still reach into it.
     if (split > 1) cluster_arrive();
     const uint32_t tmem_base = *s_tmem;
-    const int first = blockIdx.x / split, step = gridDim.x / split;
     bool joined = split == 1, left = split == 1;      // this thread has waited for the first, has arrived at the second
 
     if (warp == 0) {
@@ -175,16 +222,11 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
         bool ok = true;
         uint32_t asked = 0;
         for (int tile = first; tile < a.tiles && ok; tile += step) {
-            const int n0 = tile / a.t_tiles * kRows, t0 = tile % a.t_tiles * NT;
             for (int kb = kb0; kb < kb1; kb++, st.next(), asked++) {
+                if (asked < (uint32_t)early) continue;
                 ok = mbar_wait_warp(EMPTY(st.i), st.round ^ 1, s_abort, a.err);
                 if (!ok) break;
-                if (elect_one()) {
-                    const uint32_t dst = smem_u32(ring + st.i * S::kStage);
-                    mbar_expect_tx(FULL(st.i), S::kStage);      // what a box reads past the matrix is zero and counts all the same
-                    tma_load_2d(dst, &tmap_w, kb * kFp8Block, n0, FULL(st.i));
-                    if (!FUSED) tma_load_2d(dst + kWBytes, &tmap_a, kb * kFp8Block, t0, FULL(st.i));
-                }
+                if (elect_one()) load(st.i, tile, kb);
                 __syncwarp();
             }
         }
@@ -192,15 +234,15 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
         if (!ok)
             for (uint32_t j = asked > (uint32_t)a.stages ? asked - a.stages : 0; j < asked; j++)
                 for (uint32_t i = 0; i < kSpin && !mbar_try_wait(FULL(j % a.stages), (j / a.stages) & 1); i++) {}
-    } else if (warp == 1) {
+    } else if (warp == 1 || warp == 3) {
+        // two issuers take the blocks in turn: what a wait and the issue cost one of them passes while the other issues
         Ring st(a.stages), p(S::kAcc);
-        bool ok = !FUSED || mbar_wait_warp(CODES, 0, s_abort, a.err), seen = false;
+        bool ok = true, my_turn = warp == 1;
         for (int tile = first; tile < a.tiles && ok; tile += step) {
-            for (int i = 0; i < nkb; i++) {
-                if (!seen) {
-                    ok = mbar_wait_warp(ACC_EMPTY(p.i), p.round ^ 1, s_abort, a.err) && mbar_wait_warp(FULL(st.i), st.round, s_abort, a.err);
-                    if (!ok) break;
-                }
+            for (int i = 0; i < nkb; i++, st.next(), p.next(), my_turn = !my_turn) {
+                if (!my_turn) continue;
+                ok = mbar_wait_warp(ACC_EMPTY(p.i), p.round ^ 1, s_abort, a.err) && mbar_wait_warp(FULL(st.i), st.round, s_abort, a.err);
+                if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t wsm = smem_u32(ring + st.i * S::kStage);
                 const uint64_t wdesc = umma_desc(wsm), adesc = umma_desc(FUSED ? smem_u32(codes + i * S::kABytes) : wsm + kWBytes);
@@ -211,17 +253,13 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
                     umma_commit(ACC_FULL(p.i));
                 }
                 __syncwarp();
-                st.next();
-                p.next();
-                // a look at the next block's barriers while these products run
-                seen = __all_sync(0xffffffffu, mbar_test_wait(ACC_EMPTY(p.i), p.round ^ 1) & mbar_test_wait(FULL(st.i), st.round));
             }
         }
     } else if (warp == 2) {
         // slots of scales, four blocks asked for at a time and the next four before these are handed out
         constexpr int kPer = (NT + 31) / 32, kAhead = 4;
         Ring p(S::kAcc);
-        bool ok = !FUSED || mbar_wait_warp(CODES, 0, s_abort, a.err);
+        bool ok = true;
         float now[kAhead][kPer], next[kAhead][kPer];
         for (int tile = first; tile < a.tiles && ok; tile += step) {
             const int nb = tile / a.t_tiles, t0 = tile % a.t_tiles * NT;
@@ -261,40 +299,6 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
         }
     } else if (warp >= 4) {
         const int etid = threadIdx.x - 128, quarter = warp & 3, col0 = (warp - 4) / 4 * S::kCols;
-        if (FUSED) {
-            // rows past M are zero
-            for (int w = etid; w < nkb * (NT * 8); w += 32 * (S::kEpi + S::kHelp))
-                if (w / 8 % NT >= a.M) *reinterpret_cast<uint4*>(codes + w * 16) = make_uint4(0, 0, 0, 0);
-            // sixteen lanes quantise one block of one row, eight elements each, into its place of the swizzled operand; all of a
-            // pass's rows are asked for before the first is used
-            constexpr int kGroups = 2 * (S::kEpi + S::kHelp), kAtOnce = 4;
-            const int piece = lane % 16, units = nkb * a.M;
-            const uint32_t by_m = 65536u / a.M + 1;      // (w * by_m) >> 16 = w / M for w < 65536 / M
-            for (int w0 = etid / 32 * 2; w0 < units; w0 += kGroups * kAtOnce) {
-                float f[kAtOnce][8], sc[kAtOnce];
-                uint2 q[kAtOnce];
-                int at[kAtOnce], row[kAtOnce];
-#pragma unroll
-                for (int u = 0; u < kAtOnce; u++) {
-                    const int w = w0 + lane / 16 + u * kGroups, i = (w * by_m) >> 16, r = w - i * a.M, k = (kb0 + i) * kFp8Block + piece * 8;
-                    const int valid = w < units ? a.K - k : 0;
-                    at[u] = i, row[u] = r;
-                    if (a.x_dtype == 0)
-                        fp8_load8(reinterpret_cast<const __nv_bfloat16*>(a.x) + r * a.x_stride + k, a.x_vec, valid, f[u]);
-                    else
-                        fp8_load8(reinterpret_cast<const float*>(a.x) + r * a.x_stride + k, a.x_vec, valid, f[u]);
-                }
-                fp8_encode(f, q, sc);
-#pragma unroll
-                for (int u = 0; u < kAtOnce; u++) {
-                    if (w0 + lane / 16 + u * kGroups >= units) continue;
-                    *reinterpret_cast<uint2*>(codes + at[u] * S::kABytes + row[u] * 128 + (((piece >> 1) ^ (row[u] & 7)) << 4) + (piece & 1) * 8) = q[u];
-                    if (piece == 0) row_scales[at[u] * NT + row[u]] = sc[u];
-                }
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // the tensor core reads these bytes
-            mbar_arrive_warp(CODES);
-        }
         Ring p(S::kAcc);
         uint32_t done = 0, got = 0;
         bool ok = true;
@@ -344,19 +348,22 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
                 }
                 continue;
             }
-            // the cluster's sums: token j belongs to the CTA j / share (a power of two)
-            const int log_share = __ffs(NT / split) - 1, share = NT / split, mine = min(share, a.M - t0 - rank * share);
+            // the cluster's sums: token j belongs to the CTA j / share
+            const int share = (NT + split - 1) / split, mine = min(min(share, NT - rank * share), a.M - t0 - rank * share);
             const bool last = tile + step >= a.tiles;
             if (etid == 0 && mine > 0) mbar_expect_tx(SUM_FULL, split * mine * kRows * 4);
             if (!joined) cluster_join(), joined = true;
             if (done > 0) ok = __all_sync(0xffffffffu, cluster_wait(SUM_FREE, (done - 1) & 1, s_abort, a.err));
             if (!ok) break;
-            const uint32_t to_sums = smem_u32(sums + rank * share * kRows + row);
+            const uint32_t my_sums = smem_u32(sums + rank * share * kRows + row);
+            uint32_t to_sums = 0, to_bar = 0;
+            int to = col0 / share, in_share = col0 - to * share;
 #pragma unroll
             for (int j = 0; j < S::kCols; j++) {
-                const int col = col0 + j, to = col >> log_share;
-                if (t0 + col < a.M)
-                    remote_store(map_shared_to(to_sums + (col & (share - 1)) * kRows * 4, to), acc[j], map_shared_to(SUM_FULL, to));
+                if (t0 + col0 + j >= a.M) break;
+                if (j == 0 || in_share == 0) to_sums = map_shared_to(my_sums, to), to_bar = map_shared_to(SUM_FULL, to);
+                remote_store(to_sums + in_share * kRows * 4, acc[j], to_bar);
+                if (++in_share == share) in_share = 0, to++;
             }
             __syncwarp();
             if (last) cluster_arrive(), left = true;      // nothing of this warp's goes to another CTA from here on
@@ -377,11 +384,11 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
             if (!last && lane < split) remote_arrive(map_shared_to(SUM_FREE, lane));
         }
     }
+    if (!joined) cluster_join();
+    if (!left) cluster_arrive();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "n"(S::kTmem) : "memory");
-    if (!joined) cluster_join();
-    if (!left) cluster_arrive();
     if (split > 1) cluster_join();
 }
 
@@ -397,29 +404,36 @@ bool make_codes_map(CUtensorMap* map, const void* base, int64_t rows, int64_t K,
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-constexpr size_t kSmemLimit = 227 * 1024;
-
 template <int NT, bool FUSED>
 int launch(const uint8_t* codes, const uint8_t* w, Fp8Args a, int sm_count, cudaStream_t s) {
     using S = Shape<NT, FUSED>;
     a.blocks = (a.K + kFp8Block - 1) / kFp8Block;
     a.t_tiles = (a.M + NT - 1) / NT;
     a.tiles = a.t_tiles * ((a.N + kRows - 1) / kRows);
-    // too few tiles for the SMs: two to eight CTAs share a tile's blocks, two blocks each at least
+    // Too few tiles to keep every SM loading: the CTAs of a cluster share a tile's blocks.  The busiest SM's blocks are what a call
+    // waits for; joining the sums costs about as much as three blocks.
     int split = 1;
-    while (split < kMaxSplit && (long long)a.tiles * split * 2 <= sm_count && a.blocks >= split * 4) split *= 2;
+    long long best = 0;
+    for (int q = 1; q <= kMaxSplit && q <= a.blocks; q++) {
+        if (q > 1 && (long long)a.tiles * q > (q <= 4 ? S::kPerSm * sm_count : S::kPerSm * sm_count * 7 / 8)) break;     // larger clusters do not fill every SM
+        const long long cost = ((long long)a.tiles * q + sm_count - 1) / sm_count * ((a.blocks + q - 1) / q) + (q > 1 ? 3 : 0);
+        if (q == 1 || cost < best) best = cost, split = q;
+    }
     const int fused_blocks = (a.blocks + split - 1) / split;
+    // FUSED with many blocks to a CTA: its codes leave room for two boxes beside a second CTA, or the SM is its own
+    size_t room = S::kSmem;
+    if (S::bytes(3, split, fused_blocks) > room) room = 227 * 1024;
     a.stages = kMaxStages;
-    while (a.stages > 2 && S::bytes(a.stages, split, fused_blocks) > kSmemLimit) a.stages--;
+    while (a.stages > 2 && S::bytes(a.stages, split, fused_blocks) > room) a.stages--;
     const size_t smem = S::bytes(a.stages, split, fused_blocks);
     CUtensorMap map_w, map_a;
     if (!make_codes_map(&map_w, w, a.N, a.K, kRows) || (!FUSED && !make_codes_map(&map_a, codes, a.M, a.K, NT))) return -(int)cudaErrorInvalidValue;
     if (FUSED) map_a = map_w;
     static PerDeviceOnce once;
-    cudaError_t e = allow_dyn_smem(once, fp8_umma_kernel<NT, FUSED>, kSmemLimit);
+    cudaError_t e = allow_dyn_smem(once, fp8_umma_kernel<NT, FUSED>, 227 * 1024);
     if (e != cudaSuccess) return -(int)e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(split * max(1, min(a.tiles, sm_count / split)));
+    cfg.gridDim = dim3(split * max(1, min(a.tiles, S::kPerSm * sm_count / split)));
     cfg.blockDim = dim3(S::kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;

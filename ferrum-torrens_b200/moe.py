@@ -15,6 +15,7 @@ computation goes through the library, which has no CPU path.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import os
 import sys
 from dataclasses import dataclass
@@ -622,90 +623,95 @@ class B200MoE:
         return c
 
     # -- block-scaled 8-bit products ------------------------------------------------------------
+    # A decode step makes these calls by the hundred, and their kernels take a few microseconds: the checks below are one
+    # expression per tensor, and only a refusal looks for its reason.
     def _on(self, stream) -> int:
         """The stream of a call: the given one, else the current one of this adapter's device."""
         if stream is None:
-            return _torch().cuda.current_stream(self.device).cuda_stream
+            return _current_stream()(self.device)
         return stream if isinstance(stream, int) else stream.cuda_stream
 
-    def _rows(self, t, what: str, dtypes, shape=None) -> int:
-        """Address of a tensor on this adapter's device whose last dimension is contiguous; its rows may be apart."""
-        if t.dtype not in dtypes:
-            raise bad(f"{what} cannot be {t.dtype}")
-        if t.device.type != "cuda" or t.device.index != self.device:
-            raise bad(f"{what} must be on device {self.device}, not {t.device}")
-        if t.dim() != 2 or (shape is not None and tuple(t.shape) != shape):
-            raise bad(f"{what} is {tuple(t.shape)}, expected {shape if shape is not None else 'two dimensions'}")
-        if t.shape[1] > 1 and t.stride(1) != 1:
-            raise bad(f"{what} must be contiguous in its last dimension")
-        return t.data_ptr()
+    def _rows(self, t, what: str, codes: dict, shape=None) -> int:
+        """Address of a matrix on this adapter's device whose last dimension is contiguous; its rows may be apart."""
+        if (t.dtype in codes and t.get_device() == self.device and t.dim() == 2 and (shape is None or t.shape == shape)
+                and (t.stride(1) == 1 or t.shape[1] <= 1)):
+            return t.data_ptr()
+        raise self._refusal(t, what, codes, shape if shape is not None else "two dimensions", "contiguous in its last dimension")
 
-    def _flat(self, t, what: str, dtypes, shape) -> int:
+    def _flat(self, t, what: str, codes: dict, shape) -> int:
         """Address of a contiguous tensor of this shape on this adapter's device."""
-        if t.dtype not in dtypes:
-            raise bad(f"{what} cannot be {t.dtype}")
-        if t.device.type != "cuda" or t.device.index != self.device:
-            raise bad(f"{what} must be on device {self.device}, not {t.device}")
-        if tuple(t.shape) != shape:
-            raise bad(f"{what} is {tuple(t.shape)}, expected {shape}")
-        if not t.is_contiguous():
-            raise bad(f"{what} must be contiguous")
-        return t.data_ptr()
+        if t.dtype in codes and t.get_device() == self.device and t.shape == shape and t.is_contiguous():
+            return t.data_ptr()
+        raise self._refusal(t, what, codes, shape, "contiguous")
+
+    def _refusal(self, t, what: str, codes: dict, shape, order: str) -> MoEError:
+        if t.dtype not in codes:
+            return bad(f"{what} cannot be {t.dtype}")
+        if t.get_device() != self.device:
+            return bad(f"{what} must be on device {self.device}, not {t.device}")
+        if t.shape != shape and (t.dim() != 2 or not isinstance(shape, str)):
+            return bad(f"{what} is {tuple(t.shape)}, expected {shape}")
+        return bad(f"{what} must be {order}")
 
     def fp8_quantize(self, x, out=None, stream=None):
         """Rows of bf16 or f32 to e4m3 with one scale for each block of 128: returns (codes [M, K] float8_e4m3fn, scales
         [ceil(K / 128), M] f32).  K a multiple of 16; the rows of x may be apart.  `out`: both tensors, to be written."""
-        torch = _torch()
-        px = self._rows(x, "x", (torch.bfloat16, torch.float32))
+        ty = _types()
+        px = self._rows(x, "x", ty.act)
         m, k = x.shape
-        blocks = -(-k // 128)
-        if out is None:
-            out = (torch.empty((m, k), dtype=torch.float8_e4m3fn, device=x.device),
-                   torch.empty((blocks, m), dtype=torch.float32, device=x.device))
-        q, scale = out
-        pq = self._flat(q, "the codes", (torch.float8_e4m3fn,), (m, k))
-        ps = self._flat(scale, "the scales", (torch.float32,), (blocks, m))
-        self._check(self._lib.ftm_fp8_quantize(self._h, px, _dtype_code(x), m, k, _row_stride(x), pq, ps, self._on(stream)))
-        return q, scale
+        q, scale = out = self._fp8_pair(x, m, k) if out is None else out
+        pq = self._flat(q, "the codes", ty.e4m3, (m, k))
+        ps = self._flat(scale, "the scales", ty.f32, (-(-k // 128), m))
+        rc = self._lib.ftm_fp8_quantize(self._h, px, ty.act[x.dtype], m, k, x.stride(0) if m > 1 else k, pq, ps, self._on(stream))
+        if rc:
+            self._check(rc)
+        return out
 
     def fp8_gemm(self, a, a_scale, w, w_scale, out, stream=None):
         """out [M, N] (bf16 or f32) = a [M, K] @ w [N, K]^T of e4m3 codes, with the scales fp8_quantize gives a_scale
         [ceil(K / 128), M] and one per 128 x 128 block of the weight, w_scale [ceil(N / 128), ceil(K / 128)] f32."""
-        torch = _torch()
-        e4m3, f32 = (torch.float8_e4m3fn,), (torch.float32,)
-        m, n, k, pw, pws, pc = self._fp8_operands(a, w, w_scale, out)
-        pa = self._flat(a, "a", e4m3, (m, k))
-        pas = self._flat(a_scale, "the scales of a", f32, (-(-k // 128), m))
-        self._check(self._lib.ftm_fp8_gemm(self._h, pa, pas, pw, pws, m, n, k, pc, _dtype_code(out), _row_stride(out), self._on(stream)))
+        ty = _types()
+        m, n, k, blocks, pw, pws, pc = self._fp8_operands(ty, a, w, w_scale, out)
+        pa = self._flat(a, "a", ty.e4m3, (m, k))
+        pas = self._flat(a_scale, "the scales of a", ty.f32, (blocks, m))
+        rc = self._lib.ftm_fp8_gemm(self._h, pa, pas, pw, pws, m, n, k, pc, ty.act[out.dtype], out.stride(0) if m > 1 else n, self._on(stream))
+        if rc:
+            self._check(rc)
         return out
 
     def fp8_linear(self, x, w, w_scale, out, scratch=None, stream=None):
-        """out [M, N] = fp8_gemm of fp8_quantize(x): x [M, K] bf16 or f32 (rows may be apart), the rest as for fp8_gemm.
-        `scratch`: a pair as fp8_quantize returns it for x, kept by the caller (made here when it is None)."""
-        torch = _torch()
-        px = self._rows(x, "x", (torch.bfloat16, torch.float32))
-        m, n, k, pw, pws, pc = self._fp8_operands(x, w, w_scale, out)
-        blocks = -(-k // 128)
-        if scratch is None:
-            scratch = (torch.empty((m, k), dtype=torch.float8_e4m3fn, device=x.device),
-                       torch.empty((blocks, m), dtype=torch.float32, device=x.device))
-        pq = self._flat(scratch[0], "the codes", (torch.float8_e4m3fn,), (m, k))
-        ps = self._flat(scratch[1], "the scales", (torch.float32,), (blocks, m))
-        self._check(self._lib.ftm_fp8_linear(self._h, px, _dtype_code(x), _row_stride(x), pw, pws, m, n, k, pq, ps, pc, _dtype_code(out),
-                                             _row_stride(out), self._on(stream)))
+        """out [M, N] = fp8_gemm of fp8_quantize(x): x [M, K] bf16 or f32 (rows may be apart), the rest as for fp8_gemm.  Up to
+        16 rows of up to 8192 elements are one kernel; above, `scratch` is a pair as fp8_quantize returns it for x, kept
+        by the caller (made here when it is None)."""
+        ty = _types()
+        px = self._rows(x, "x", ty.act)
+        m, n, k, blocks, pw, pws, pc = self._fp8_operands(ty, x, w, w_scale, out)
+        if scratch is None and (m > 16 or k > 8192):
+            scratch = self._fp8_pair(x, m, k)
+        pq = ps = None
+        if scratch is not None:
+            pq = self._flat(scratch[0], "the codes", ty.e4m3, (m, k))
+            ps = self._flat(scratch[1], "the scales", ty.f32, (blocks, m))
+        rc = self._lib.ftm_fp8_linear(self._h, px, ty.act[x.dtype], x.stride(0) if m > 1 else k, pw, pws, m, n, k, pq, ps, pc, ty.act[out.dtype],
+                                      out.stride(0) if m > 1 else n, self._on(stream))
+        if rc:
+            self._check(rc)
         return out
 
-    def _fp8_operands(self, a, w, w_scale, out):
-        """Sizes and addresses that fp8_gemm and fp8_linear have in common."""
+    def _fp8_pair(self, x, m: int, k: int):
+        """Room for the codes and scales of m rows of k."""
         torch = _torch()
+        return (torch.empty((m, k), dtype=torch.float8_e4m3fn, device=x.device),
+                torch.empty((-(-k // 128), m), dtype=torch.float32, device=x.device))
+
+    def _fp8_operands(self, ty, a, w, w_scale, out):
+        """Sizes and addresses that fp8_gemm and fp8_linear have in common."""
         if a.dim() != 2 or w.dim() != 2 or a.shape[1] != w.shape[1]:
             raise bad(f"fp8: a weight [N, K] is wanted for rows [M, K], got {tuple(w.shape)} for {tuple(a.shape)}")
-        m, k = a.shape
-        n = w.shape[0]
-        pw = self._flat(w, "the weight", (torch.float8_e4m3fn,), (n, k))
-        pws = self._flat(w_scale, "the weight's scales", (torch.float32,), (-(-n // 128), -(-k // 128)))
-        pc = self._rows(out, "the output", (torch.bfloat16, torch.float32), (m, n))
-        return m, n, k, pw, pws, pc
+        n, k = w.shape
+        m, blocks = a.shape[0], -(-k // 128)
+        return (m, n, k, blocks, self._flat(w, "the weight", ty.e4m3, (n, k)), self._flat(w_scale, "the weight's scales", ty.f32, (-(-n // 128), blocks)),
+                self._rows(out, "the output", ty.act, (m, n)))
 
     # -- what a server reads off its logits -----------------------------------------------------
     def logprobs(self, logits, ids=None, top_n: int = 0, out=None, stream=None):
@@ -713,32 +719,51 @@ class B200MoE:
         f32, entropy [T] f32, rank [T] i32, ids of the top_n most probable [T, top_n] i32, their log probabilities [T, top_n] f32).
         A negative id asks for nothing (0, rank -1); without `ids` the first and third are None.  Equal values go by their
         index.  `out`: those five tensors, to be written; one that is None there is not computed."""
-        torch = _torch()
-        f32, i32 = (torch.float32,), (torch.int32,)
-        px = self._rows(logits, "the logits", (torch.bfloat16, torch.float32))
+        ty = _types()
+        px = self._rows(logits, "the logits", ty.act)
         rows, vocab = logits.shape
         if not 0 <= top_n <= 32:
             raise bad(f"logprobs: {top_n} alternatives (at most 32)")
         if out is None:
+            torch = _torch()
             new = lambda dtype, *shape: torch.empty(shape, dtype=dtype, device=logits.device)
             out = (new(torch.float32, rows) if ids is not None else None, new(torch.float32, rows),
                    new(torch.int32, rows) if ids is not None else None, new(torch.int32, rows, top_n), new(torch.float32, rows, top_n))
         lp, entropy, rank, top_ids, top_lp = out
-        pi = None if ids is None else self._flat(ids, "the token ids", (torch.int32, torch.int64), (rows,))
-        p1 = None if lp is None else self._flat(lp, "the log probabilities", f32, (rows,))
-        p2 = None if entropy is None else self._flat(entropy, "the entropies", f32, (rows,))
-        p3 = None if rank is None else self._flat(rank, "the ranks", i32, (rows,))
-        p4 = None if top_ids is None else self._flat(top_ids, "the alternatives", i32, (rows, top_n))
-        p5 = None if top_lp is None else self._flat(top_lp, "the alternatives' log probabilities", f32, (rows, top_n))
-        self._check(self._lib.ftm_logprobs(self._h, px, _dtype_code(logits), rows, vocab, _row_stride(logits), pi,
-                                           L.I32 if ids is None else _dtype_code(ids), top_n, p1, p2, p3, p4, p5, self._on(stream)))
+        flat, shape = self._flat, (rows,)
+        pi = None if ids is None else flat(ids, "the token ids", ty.ids, shape)
+        p1 = None if lp is None else flat(lp, "the log probabilities", ty.f32, shape)
+        p2 = None if entropy is None else flat(entropy, "the entropies", ty.f32, shape)
+        p3 = None if rank is None else flat(rank, "the ranks", ty.i32, shape)
+        p4 = None if top_ids is None else flat(top_ids, "the alternatives", ty.i32, (rows, top_n))
+        p5 = None if top_lp is None else flat(top_lp, "the alternatives' log probabilities", ty.f32, (rows, top_n))
+        rc = self._lib.ftm_logprobs(self._h, px, ty.act[logits.dtype], rows, vocab, logits.stride(0) if rows > 1 else vocab, pi,
+                                    L.I32 if ids is None else ty.ids[ids.dtype], top_n, p1, p2, p3, p4, p5, self._on(stream))
+        if rc:
+            self._check(rc)
         return out
 
 
-def _row_stride(t) -> int:
-    """Elements between the rows of a matrix; a single row has none."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+class _Types:
+    """The dtype codes each kind of tensor may have."""
 
+    def __init__(self, torch):
+        self.act = {torch.bfloat16: L.BF16, torch.float32: L.F32}
+        self.f32, self.i32 = {torch.float32: L.F32}, {torch.int32: L.I32}
+        self.ids = {torch.int32: L.I32, torch.int64: L.I64}
+        self.e4m3 = {torch.float8_e4m3fn: None}
+
+
+@functools.lru_cache(maxsize=None)
+def _types() -> _Types:
+    return _Types(_torch())
+
+
+@functools.lru_cache(maxsize=None)
+def _current_stream():
+    """ordinal -> handle of that device's current stream, without an object in between where torch offers it."""
+    torch = _torch()
+    return getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda ordinal: torch.cuda.current_stream(ordinal).cuda_stream)
 
 
 def _check_device_step(step: MoEDeviceRequest) -> int:
