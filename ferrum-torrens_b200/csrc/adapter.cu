@@ -1360,7 +1360,7 @@ FTM_API int ftm_logprobs(ftm_handle* h, const void* logits, int dtype, int32_t r
         !aligned_to(entropy_out, 4) || !aligned_to(rank_out, 4) || !aligned_to(top_ids_out, 4) || !aligned_to(top_logprobs_out, 4))
         return fail(h, FTM_ERR_BAD, "moe: logprobs: a buffer is not aligned to its type");
     return count_launches(h, launch_logprobs(logits, dtype, rows, vocab, row_stride, ids, ids_dtype, top_n, logprob_out, entropy_out, rank_out,
-                                             top_ids_out, top_logprobs_out, h->sm_total, h->flags + 4, h->ctx(pick(h, stream))), "logprobs");
+                                             top_ids_out, top_logprobs_out, h->sm_total, h->flags + 4, h->flags + 2, h->ctx(pick(h, stream))), "logprobs");
 }
 
 }  // extern "C"

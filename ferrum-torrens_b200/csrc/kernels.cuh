@@ -269,6 +269,6 @@ int launch_fp8_linear(const void* x, int x_dtype, long long x_stride, const uint
 // logprobs.cu: what a server reads off its logits; a negative result is a CUDA error code
 int launch_logprobs(const void* logits, int dtype, int rows, int vocab, long long stride, const void* ids, int ids_dtype, int top_n,
                     float* logprob, float* entropy, int32_t* rank, int32_t* top_ids, float* top_logprobs, int sm_count,
-                    int32_t* bad_flag, const Ctx& c);
+                    int32_t* bad_flag, int32_t* err, const Ctx& c);
 
 }  // namespace ftm

@@ -9,18 +9,17 @@
 // maximum rises (t gains s * (old - new)); the partial triples are joined over the warp, the CTA and the cluster.
 // Differences are clamped at -1e20: an element of -inf adds e^d = 0 times a finite d; NaN and +inf make s a NaN.
 //
-// Alternatives (n <= 32).  The pass itself only notes the maximum of every warp's part of every tile.  Then every warp publishes
-// the largest of its lanes' maxima over the whole row, k of them with 8 k >= n, and the n-th largest of what is published is a
-// bound: n elements reach it, so what is below cannot belong to the answer.  The few tiles whose maximum reaches it are read again
-// (from L2), the elements that reach it are collected and placed by counting the better ones.  Where ties make them too
-// many, every warp keeps its n best as a sorted list over its lanes instead.
+// Alternatives (n <= 32).  The pass itself only notes the maximum of every warp's part of every tile.  The 256 lanes' maxima,
+// taken together by fours, give 64 values, and the n-th largest of these is a bound: n elements reach it, so what is below
+// cannot belong to the answer.  The tiles whose maximum reaches it are read again (from L2 mostly), the elements that reach it
+// are collected and placed by counting the better ones.  Where ties make them too many, every warp keeps its n best as
+// a sorted list over its lanes instead.
 //
 // Rank: a lane counts in a tile only if its maximum there reaches the token's value; bf16 pairs are compared as they are.
 //
-// A row is split over the CTAs of a cluster when there are few rows; results meet in the first CTA's shared memory, so
-// no workspace in global memory is needed and calls on several streams share nothing.
+// Rows of small batches are split over the CTAs of a cluster, so that every SM loads; results are sent to the first CTA's shared memory, so no workspace in global memory is needed and calls on
+// several streams share nothing.
 #include <climits>
-#include <cooperative_groups.h>
 
 #include "kernels.cuh"
 
@@ -28,18 +27,19 @@ namespace ftm {
 
 namespace {
 
-namespace cg = cooperative_groups;
-
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMaxCluster = 16;      // more than 8 CTAs need the opt-in of launch_logprobs
-constexpr int kVecs = 4;             // 128-bit loads of a thread per tile
+constexpr int kVecs = 4;             // 128-bit words of a lane per tile
+constexpr int kWarpVecs = 32 * kVecs;        // 128-bit words of a warp per tile
+constexpr int kTileVecs = kWarps * kWarpVecs;
+constexpr int kTileBytes = kTileVecs * 16;   // 16 KiB
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kInf = __builtin_huge_valf();
 constexpr float kFar = -1e20f;       // differences below this have exponential 0; clamped there, sums of them stay finite
-constexpr int kCandidates = 1024;
-constexpr int kNotes = 64;           // noted maxima of a warp; longer rows note several tiles together
-constexpr int kPublish = 8;          // values that a warp can publish
+constexpr int kCandidates = 512;
+constexpr int kNotes = 32;           // noted maxima of a warp; longer parts note several tiles together
+constexpr uint32_t kSpin = 1u << 20; // looks at a barrier before a wait is given up
 
 __device__ __forceinline__ float ex2(float v) {
     float r;
@@ -99,15 +99,26 @@ struct Word<float> {
     __device__ __forceinline__ static float largest(uint32_t w) { return __uint_as_float(w); }
     __device__ __forceinline__ static uint32_t all(float v) { return __float_as_uint(v); }
     __device__ __forceinline__ static bool any_reaches(uint32_t w, uint32_t v) { return __uint_as_float(w) >= __uint_as_float(v); }
-    __device__ __forceinline__ static float get(uint32_t w, int) { return __uint_as_float(w); }
-    // how many elements of four words are above v, added to a tile's count
-    using Count = int;
-    __device__ __forceinline__ static void count_above(const uint4& w, uint32_t v, int& count) {
-        const float f = __uint_as_float(v);
-        count += (__uint_as_float(w.x) > f) + (__uint_as_float(w.y) > f) + (__uint_as_float(w.z) > f) + (__uint_as_float(w.w) > f);
+    // one bit for each element of four words that is v or more
+    __device__ __forceinline__ static uint32_t reaching(const uint4& w, uint32_t v) {
+        return any_reaches(w.x, v) | any_reaches(w.y, v) << 1 | any_reaches(w.z, v) << 2 | any_reaches(w.w, v) << 3;
     }
-    __device__ __forceinline__ static int none() { return 0; }
-    __device__ __forceinline__ static int total(int count) { return count; }
+    // how many elements of four words are above v, added to a tile's counts of even and odd elements
+    using Count = uint64_t;
+    __device__ __forceinline__ static float above(uint32_t w, float v) {
+        float r;
+        asm("set.gt.f32.f32 %0, %1, %2;" : "=f"(r) : "f"(__uint_as_float(w)), "f"(v));
+        return r;
+    }
+    __device__ __forceinline__ static void count_above(const uint4& w, uint32_t v, uint64_t& count) {
+        const float f = __uint_as_float(v);
+        count = add2(count, add2(pair(above(w.x, f), above(w.y, f)), pair(above(w.z, f), above(w.w, f))));
+    }
+    __device__ __forceinline__ static uint64_t none() { return 0; }
+    __device__ __forceinline__ static int total(uint64_t count) {
+        const float2 c = unpair(count);
+        return (int)(c.x + c.y);
+    }
     // the largest value below v (not -inf): what is above it is v or more
     __device__ __forceinline__ static float below(float v) { return nextafterf(v, -kInf); }
 };
@@ -126,7 +137,12 @@ struct Word<__nv_bfloat16> {
     }
     __device__ __forceinline__ static uint32_t all(float v) { return (__float_as_uint(v) >> 16) * 0x10001u; }      // (v is a bf16 value)
     __device__ __forceinline__ static bool any_reaches(uint32_t w, uint32_t v) { return __hge2_mask(as2(w), as2(v)) != 0; }
-    __device__ __forceinline__ static float get(uint32_t w, int e) { return bf16_bits_to_f32(e ? w >> 16 : w & 0xffffu); }
+    __device__ __forceinline__ static uint32_t reaching(const uint4& w, uint32_t v) {
+        const uint32_t a = __hge2_mask(as2(w.x), as2(v)) & 0x00020001u, b = __hge2_mask(as2(w.y), as2(v)) & 0x00080004u;
+        const uint32_t c = __hge2_mask(as2(w.z), as2(v)) & 0x00200010u, d = __hge2_mask(as2(w.w), as2(v)) & 0x00800040u;
+        const uint32_t m = a | b | c | d;
+        return (m | m >> 16) & 0xffu;
+    }
     using Count = __nv_bfloat162;      // (a tile's counts of even and odd elements are whole numbers that a bf16 holds)
     __device__ __forceinline__ static void count_above(const uint4& w, uint32_t v, __nv_bfloat162& count) {
         count = __hadd2(count, __hadd2(__hadd2(__hgt2(as2(w.x), as2(v)), __hgt2(as2(w.y), as2(v))), __hadd2(__hgt2(as2(w.z), as2(v)), __hgt2(as2(w.w), as2(v)))));
@@ -145,7 +161,8 @@ struct Stats {
 
     // distance from the maximum `top` that this one is joined under: 0 where nothing was summed (or a NaN, which stays)
     __device__ __forceinline__ float below(float top) const { return m == -kInf ? 0.f : max_nan(m - top, kFar); }
-    __device__ __forceinline__ void rise(float mx) {       // the maximum may rise to mx
+    // the maximum may rise to mx.  (The lanes of a warp share theirs, so that the branch is taken by all or none.)
+    __device__ __forceinline__ void rise(float mx) {
         if (mx > m) {
             const float d = below(mx), f = ex2(d * kLog2e);
             t = f * (t + s * d);
@@ -180,73 +197,127 @@ struct Stats {
         s += e;
         t = fmaf(e, d, t);
     }
-    __device__ __forceinline__ void join(float m2, float s2, float t2) {
-        Stats o;
-        o.m = m2, o.s = s2, o.t = t2;
-        const float top = fmaxf(m, m2);
-        const float d1 = below(top), d2 = o.below(top);
-        const float f1 = ex2(d1 * kLog2e), f2 = ex2(d2 * kLog2e);
-        t = f1 * (t + s * d1) + f2 * (t2 + s2 * d2);
-        s = f1 * s + f2 * s2;
-        m = top;
-    }
+    // the lanes' statistics joined, in every lane
     __device__ __forceinline__ void join_warp() {
+        const float top = from_ordered(__reduce_max_sync(0xffffffffu, ordered(m)));
+        const float d = below(top), f = ex2(d * kLog2e);
+        t = f * (t + s * d);
+        s *= f;
+        m = top;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
-            const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o), t2 = __shfl_xor_sync(0xffffffffu, t, o);
-            join(m2, s2, t2);
+            s += __shfl_xor_sync(0xffffffffu, s, o);
+            t += __shfl_xor_sync(0xffffffffu, t, o);
         }
     }
 };
 
-__device__ __forceinline__ bool better(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
+// An element as one whole number, larger for what comes first: the value in the order of the floats (the two zeros as one),
+// then the lower index.  0 is no element.
+__device__ __forceinline__ uint64_t key_of(float v, int i) {
+    return (uint64_t)((uint32_t)ordered(v + 0.f) ^ 0x80000000u) << 32 | (uint32_t)~i;
+}
+__device__ __forceinline__ float key_value(uint64_t k) { return from_ordered((int)((uint32_t)(k >> 32) ^ 0x80000000u)); }
+__device__ __forceinline__ int key_index(uint64_t k) { return (int)~(uint32_t)k; }
 
-// a warp's sorted list, one entry per lane; empty entries are (-inf, INT_MAX)
+// A warp's n best elements, sorted, one per lane (0: none yet).
 struct TopList {
-    float v = -kInf;
-    int i = INT_MAX;
-    float last_v = -kInf;      // the n-th entry, in every lane: an element enters when it is better
-    int last_i = -1;           // (nothing that is -inf enters an empty place: those are filled in at the end)
+    uint64_t k = 0, last = 0;      // last: the n-th entry, in every lane
 
-    __device__ __forceinline__ void insert(float x, int at, int n, int lane) {
-        const int pos = __popc(__ballot_sync(0xffffffffu, better(v, i, x, at)));
-        const float pv = __shfl_up_sync(0xffffffffu, v, 1);
-        const int pi = __shfl_up_sync(0xffffffffu, i, 1);
-        if (lane > pos) v = pv, i = pi;
-        if (lane == pos) v = x, i = at;
-        const float lv = __shfl_sync(0xffffffffu, v, n - 1);
-        const int li = __shfl_sync(0xffffffffu, i, n - 1);
-        last_v = lv;
-        last_i = lv == -kInf ? -1 : li;
-    }
-    // offers one element per lane; below `bound` nothing can belong to the answer
-    __device__ __forceinline__ void offer(float x, int at, float bound, int n, int lane) {
-        unsigned todo = __ballot_sync(0xffffffffu, x >= bound && better(x, at, last_v, last_i));
+    // offers one element per lane (0: none)
+    __device__ __forceinline__ void offer(uint64_t e, int n, int lane) {
+        unsigned todo = __ballot_sync(0xffffffffu, e > last);
         while (todo) {
-            const int src = __ffs(todo) - 1;
-            insert(__shfl_sync(0xffffffffu, x, src), __shfl_sync(0xffffffffu, at, src), n, lane);
+            const uint64_t x = __shfl_sync(0xffffffffu, e, __ffs(todo) - 1);
+            const int pos = __popc(__ballot_sync(0xffffffffu, k > x));
+            const uint64_t up = __shfl_up_sync(0xffffffffu, k, 1);
+            if (lane > pos) k = up;
+            if (lane == pos) k = x;
+            last = __shfl_sync(0xffffffffu, k, n - 1);
             todo &= todo - 1;
-            todo &= __ballot_sync(0xffffffffu, better(x, at, last_v, last_i));
+            todo &= __ballot_sync(0xffffffffu, e > last);
         }
     }
 };
 
-// place of entry (w, p) among `lists` sorted lists of n entries
-__device__ __forceinline__ int merged_place(const float (*val)[32], const int (*idx)[32], int lists, int n, int w, int p) {
-    const float v = val[w][p];
-    const int i = idx[w][p];
-    int place = p;
-    for (int q = 0; q < lists; q++) {
-        if (q == w) continue;
-        int lo = 0, hi = n;
-        while (lo < hi) {
-            const int mid = (lo + hi) / 2;
-            if (better(val[q][mid], idx[q][mid], v, i)) lo = mid + 1;
-            else hi = mid;
-        }
-        place += lo;
+// how many of `count` different keys are larger than k; `keys` has room for one key more and is aligned to 16 bytes
+__device__ __forceinline__ int larger_than(const uint64_t* keys, int count, uint64_t k) {
+    int place = 0;
+#pragma unroll 4
+    for (int o = 0; o < count; o += 2) {
+        const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(keys + o);
+        place += (v.x > k) + (int)((v.y > k) & (o + 1 < count));
     }
     return place;
+}
+
+// The best n <= 32 of up to 16 sorted lists (0 ends one), by one warp, which gets them in its lanes.  The first two entries of
+// each list, or as many as make n, give a bound that n of them reach; what reaches it is moved together and placed by
+// counting.  room: lists * 32 keys, aligned to 16 bytes; best: 32 keys.
+__device__ __forceinline__ uint64_t merge_lists(const uint64_t (*list)[32], int lists, int n, int lane, uint64_t* room, uint64_t* best) {
+    const int deep = max(2, (n + lists - 1) / lists);
+    uint64_t bound = 0;
+    if (lists * deep <= 32) {
+        const uint64_t e = lane < lists * deep ? list[lane / deep][lane % deep] : 0;
+        int place = 0;
+#pragma unroll 8
+        for (int o = 0; o < 32; o++) {
+            const uint64_t other = __shfl_sync(0xffffffffu, e, o);
+            place += (int)(other > e) | (int)((other == e) & (o < lane));
+        }
+        bound = __shfl_sync(0xffffffffu, e, __ffs(__ballot_sync(0xffffffffu, place == n - 1)) - 1);
+    }
+    int mine = 0;
+    if (lane < lists)
+        while (mine < n && list[lane][mine] >= bound && list[lane][mine] != 0) mine++;
+    int at = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int below = __shfl_up_sync(0xffffffffu, at, o);
+        if (lane >= o) at += below;
+    }
+    const int count = __shfl_sync(0xffffffffu, at, 31);
+    at -= mine;
+    for (int q = 0; q < mine; q++) room[at + q] = list[lane][q];
+    __syncwarp();
+    // (an entry's place is found by its lane; the n-th and those before it end up in the lanes)
+    best[lane] = 0;
+    __syncwarp();
+    for (int q = lane; q < count; q += 32) {
+        const uint64_t k = room[q];
+        const int place = larger_than(room, count, k);
+        if (place < n) best[place] = k;
+    }
+    __syncwarp();
+    return best[lane];
+}
+
+// ---- sending results to the first CTA of the cluster -------------------------------------------
+__device__ __forceinline__ uint32_t shared_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ uint32_t in_first_cta(uint32_t addr) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+    return r;
+}
+// a store into another CTA's shared memory that counts its bytes on a barrier there
+__device__ __forceinline__ void send(uint32_t to, uint32_t v, uint32_t bar) {
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(to), "r"(v), "r"(bar) : "memory");
+}
+
+// bounded wait for a phase of a barrier in this CTA's shared memory
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) {
+    for (uint32_t i = 0; i < kSpin; i++) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (done) return true;
+    }
+    return false;
 }
 
 struct LogprobArgs {
@@ -262,33 +333,59 @@ struct LogprobArgs {
     int32_t* top_ids;
     float* top_logprobs;
     int32_t* bad_flag;
+    int32_t* err;
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
-logprobs_kernel(LogprobArgs a) {
+__global__ void __launch_bounds__(kThreads, 4)
+logprobs_kernel(LogprobArgs a, int parts) {
     using W = Word<T>;
-    constexpr int kPer = 4 * W::kElems;           // elements of a 128-bit load
-    cg::cluster_group cluster = cg::this_cluster();
-    const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
+    constexpr int kPer = 4 * W::kElems;           // elements of a 128-bit word
     const long long row = blockIdx.x / parts;
+    const int part = blockIdx.x - (int)row * parts;        // (a cluster is one row's CTAs, in their order)
     const T* const x = reinterpret_cast<const T*>(a.logits) + row * a.stride;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, n = a.top_n;
 
-    __shared__ float l_val[kMaxCluster][32];      // sorted lists to be merged: the warps', then the cluster's
-    __shared__ int l_idx[kMaxCluster][32];
-    __shared__ float m_val[32];                   // this CTA's best
-    __shared__ int m_idx[32];
-    __shared__ float c_val[kCandidates];          // elements that reached the bound
-    __shared__ int c_idx[kCandidates];
-    __shared__ int c_count;
-    __shared__ float p_stat[kWarps][3], c_stat[3];     // m, s, t
-    __shared__ int p_rank[kWarps], c_rank;
+    __shared__ __align__(8) uint64_t arrived;     // first CTA: counts the bytes the others send
+    __shared__ uint64_t lists[kMaxCluster][32];   // first CTA: the best of every CTA of the cluster
+    __shared__ uint32_t c_all[kMaxCluster][4];    // first CTA: m, s, t and rank of every CTA
+    __shared__ uint64_t best[32];                 // this CTA's best
+    __shared__ __align__(16) uint64_t found[kCandidates];  // elements that reached the bound
+    __shared__ int c_count, s_bound;
+    __shared__ float p_stat[kWarps][3];           // m, s, t
+    __shared__ int p_rank[kWarps];
     __shared__ int note[kWarps][kNotes];          // (ordered) maxima of a warp's part of one or more tiles
-    __shared__ int share[kWarps * kPublish], s_bound;
-    for (int q = lane; q < kNotes; q += 32) note[warp][q] = ordered(-kInf);
-    if (tid == 0) c_count = 0;
-    __syncwarp();      // (a warp's notes are its own until the barrier behind the pass)
+    __shared__ __align__(16) int lane_max[kThreads];       // (ordered)
+
+    // whole 128-bit words of the row, and the elements in front of and behind them
+    const int head = min((int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)), a.vocab);
+    const int vecs = (a.vocab - head) / kPer, tail = a.vocab - head - vecs * kPer;
+    const int v0 = (int)((long long)vecs * part / parts), v1 = (int)((long long)vecs * (part + 1) / parts);
+    const uint4* const xv = reinterpret_cast<const uint4*>(x + head);
+    // tiles of this CTA, and how many are noted together
+    const int tiles = (v1 - v0 + kTileVecs - 1) / kTileVecs;
+    int together = 0;
+    while ((tiles - 1) >> together >= kNotes) together++;
+
+    // this warp's share of a tile: words first_of(tile) .. + kWarpVecs, as far as the part goes
+    auto first_of = [&](int tile) { return v0 + tile * kTileVecs + warp * kWarpVecs; };
+    uint4 next[kVecs];
+    auto fetch = [&](int tile) {
+        const int first = first_of(tile) + lane;
+#pragma unroll
+        for (int u = 0; u < kVecs; u++) next[u] = first + u * 32 < v1 ? __ldg(xv + first + u * 32) : make_uint4(W::kLowest, W::kLowest, W::kLowest, W::kLowest);
+    };
+    fetch(0);      // on its way while the token is looked up
+    if (parts > 1) {
+        if (tid == 0) {
+            const uint32_t bar = shared_addr(&arrived);
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar));
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+            if (part == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"((parts - 1) * (4 + 2 * n) * 4) : "memory");
+        }
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    }
 
     // the given token: a negative id asks for nothing, one past the vocabulary is an error
     long long id = -1;
@@ -300,63 +397,54 @@ logprobs_kernel(LogprobArgs a) {
     // in front of the token an element counts from x_id on, behind it above x_id only
     const float x_id_below = x_id > -kInf ? W::below(x_id) : -kInf;
 
-    // whole 128-bit vectors of the row, and the elements in front of and behind them
-    const int head = min((int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)), a.vocab);
-    const int vecs = (a.vocab - head) / kPer, tail = a.vocab - head - vecs * kPer;
-    const int v0 = (int)((long long)vecs * part / parts), v1 = (int)((long long)vecs * (part + 1) / parts);
-    const uint4* const xv = reinterpret_cast<const uint4*>(x + head);
-
+    for (int q = lane; q < kNotes; q += 32) note[warp][q] = ordered(-kInf);
+    if (tid == 0) c_count = 0;
+    if (tid < 32) best[tid] = 0;
     Stats st;
     int ahead = 0;
-
     auto collect = [&](float v, int at, float bound) {
         if (v >= bound && v > -kInf) {
             const int place = atomicAdd(&c_count, 1);
-            if (place < kCandidates) c_val[place] = v, c_idx[place] = at;
+            if (place < kCandidates) found[place] = key_of(v, at);
         }
     };
-    // the elements outside whole vectors: one per lane of the first CTA's first warp
+    // the elements outside whole words: one per lane of the first CTA's first warp
     const bool extra = part == 0 && warp == 0 && lane < head + tail;
     const int extra_at = lane < head ? lane : a.vocab - tail + (lane - head);
     const float extra_x = extra ? load_logit(x + extra_at) : -kInf;
-    if (extra) {
-        st.rise(extra_x);
-        st.add_one(extra_x);
-        if (asked && !low_id) ahead += extra_x > (extra_at < want ? x_id_below : x_id);
+    float lane_m = fmaxf(extra_x, -kInf);      // (a NaN is not a maximum)
+    if (extra && asked && !low_id) ahead += extra_x > (extra_at < want ? x_id_below : x_id);
+    if (part == 0 && warp == 0) {
+        st.rise(from_ordered(__reduce_max_sync(0xffffffffu, ordered(lane_m))));
+        if (extra) st.add_one(extra_x);
     }
+    __syncwarp();
 
-    // tiles of this CTA, and how many are noted together
-    constexpr int kTileVecs = kThreads * kVecs;
-    const int tiles = (v1 - v0 + kTileVecs - 1) / kTileVecs;
-    int together = 0;
-    while ((tiles - 1) >> together >= kNotes) together++;
     const uint32_t id_word = W::all(low_id ? kInf : x_id), below_word = W::all(low_id ? kInf : x_id_below);
     const float look = asked && !low_id ? x_id : kInf;
     for (int tile = 0; tile < tiles; tile++) {
-        const int first = v0 + tile * kTileVecs + tid;
         uint4 r[kVecs];
 #pragma unroll
-        for (int u = 0; u < kVecs; u++)
-            r[u] = first + u * kThreads < v1 ? __ldg(xv + first + u * kThreads) : make_uint4(W::kLowest, W::kLowest, W::kLowest, W::kLowest);
+        for (int u = 0; u < kVecs; u++) r[u] = next[u];
+        fetch(tile + 1);
         uint32_t top = W::kLowest;
 #pragma unroll
         for (int u = 0; u < kVecs; u++) top = W::larger(top, W::larger(W::larger(r[u].x, r[u].y), W::larger(r[u].z, r[u].w)));
         const float mx = W::largest(top);
-        if (n > 0) {
-            const int m = __reduce_max_sync(0xffffffffu, ordered(mx));
-            if (lane == 0) note[warp][tile >> together] = together ? max(note[warp][tile >> together], m) : m;
-        }
-        if (mx >= look) {
-            typename W::Count count = W::none();
-#pragma unroll
-            for (int u = 0; u < kVecs; u++) W::count_above(r[u], head + (first + u * kThreads) * kPer < want ? below_word : id_word, count);
-            ahead += W::total(count);
-        }
-        st.rise(mx);
+        lane_m = fmaxf(lane_m, mx);
+        const int warp_mx = __reduce_max_sync(0xffffffffu, ordered(mx));
+        if (lane == 0) note[warp][tile >> together] = together ? max(note[warp][tile >> together], warp_mx) : warp_mx;
+        st.rise(from_ordered(warp_mx));
         uint64_t s2 = 0, t2 = 0;
 #pragma unroll
         for (int u = 0; u < kVecs; u++) st.template add<T>(r[u], s2, t2);
         st.take(s2, t2);
+        if (mx >= look) {
+            typename W::Count count = W::none();
+#pragma unroll
+            for (int u = 0; u < kVecs; u++) W::count_above(r[u], head + (first_of(tile) + lane + u * 32) * kPer < want ? below_word : id_word, count);
+            ahead += W::total(count);
+        }
     }
     if (asked) {
         const int id_vec = want >= head && want < head + vecs * kPer ? (want - head) / kPer : -1;
@@ -365,29 +453,17 @@ logprobs_kernel(LogprobArgs a) {
             for (int vi = v0 + tid; vi < v1; vi += kThreads)
                 for (int e = 0; e < kPer; e++) ahead += load_logit(x + head + vi * kPer + e) > -kInf || head + vi * kPer + e < want;
             if (extra) ahead += extra_x > -kInf || extra_at < want;
-        } else if (id_vec >= v0 && id_vec < v1 && (id_vec - v0) % kThreads == tid && head + id_vec * kPer < want) {
-            // the token's own vector was counted as in front of it: the token and its equals behind it do not count
+        } else if (id_vec >= v0 && id_vec < v1 && tid == 0 && head + id_vec * kPer < want) {
+            // the token's own word was counted as in front of it: the token and its equals behind it do not count
             for (int at = want; at < head + (id_vec + 1) * kPer; at++) ahead -= load_logit(x + at) == x_id;
         }
     }
 
-    // ---- warp, CTA, cluster -------------------------------------------------------------------------
-    if (n > 0) {
-        int u = ordered(st.m);
-        const int rounds = min(kPublish, (n + kWarps - 1) / kWarps * 2);
-        for (int q = 0; q < kPublish; q++) {
-            int best = INT_MIN;
-            if (q < rounds) {
-                best = __reduce_max_sync(0xffffffffu, u);
-                if (lane == __ffs(__ballot_sync(0xffffffffu, u == best)) - 1) u = INT_MIN;
-            }
-            if (lane == 0) share[warp * kPublish + q] = best;
-        }
-    }
+    // ---- the CTA's results --------------------------------------------------------------------------
+    lane_max[tid] = ordered(lane_m);
     st.join_warp();
     ahead = __reduce_add_sync(0xffffffffu, ahead);
     if (lane == 0) p_stat[warp][0] = st.m, p_stat[warp][1] = st.s, p_stat[warp][2] = st.t, p_rank[warp] = ahead;
-    if (tid < 32) m_val[tid] = -kInf, m_idx[tid] = INT_MAX;
     __syncthreads();
     if (warp == kWarps - 1) {
         Stats all;
@@ -395,38 +471,48 @@ logprobs_kernel(LogprobArgs a) {
         if (lane < kWarps) all.m = p_stat[lane][0], all.s = p_stat[lane][1], all.t = p_stat[lane][2], sum = p_rank[lane];
         all.join_warp();
         sum = __reduce_add_sync(0xffffffffu, sum);
-        if (lane == 0) c_stat[0] = all.m, c_stat[1] = all.s, c_stat[2] = all.t, c_rank = sum;
+        if (lane == 0) {
+            c_all[part][0] = __float_as_uint(all.m), c_all[part][1] = __float_as_uint(all.s), c_all[part][2] = __float_as_uint(all.t);
+            c_all[part][3] = (uint32_t)sum;
+        }
     }
     if (n > 0) {
         if (warp == 0) {
-            // the n-th largest of the published values (two per lane)
-            int u = share[lane], w = share[lane + 32], best = INT_MIN;
-            for (int q = 0; q < n; q++) {
-                best = __reduce_max_sync(0xffffffffu, max(u, w));
-                if (lane == __ffs(__ballot_sync(0xffffffffu, u == best || w == best)) - 1) {
-                    if (u == best) u = INT_MIN;
-                    else w = INT_MIN;
-                }
+            // the n-th largest of 64 values, each the largest of four lanes' maxima, two to a lane here (equal ones in the order
+            // of all u, then all w)
+            const int4 p = *reinterpret_cast<const int4*>(lane_max + lane * 8), q = *reinterpret_cast<const int4*>(lane_max + lane * 8 + 4);
+            const int u = max(max(p.x, p.y), max(p.z, p.w)), w = max(max(q.x, q.y), max(q.z, q.w));
+            int place_u = 0, place_w = 0;
+#pragma unroll 4
+            for (int o = 0; o < 32; o++) {
+                const int ou = __shfl_sync(0xffffffffu, u, o), ow = __shfl_sync(0xffffffffu, w, o);
+                place_u += ((ou > u) | ((ou == u) & (o < lane))) + (ow > u);
+                place_w += (ou >= w) + ((ow > w) | ((ow == w) & (o < lane)));
             }
-            if (lane == 0) s_bound = max(best, ordered(-kInf));
+            if (place_u == n - 1) s_bound = u;
+            if (place_w == n - 1) s_bound = w;
         }
         __syncthreads();
         const float bound = from_ordered(s_bound);
         const uint32_t bound_word = W::all(bound);
-        for (int g = 0; g <= (tiles - 1) >> together && tiles > 0; g++) {
+        for (int g = 0; tiles > 0 && g <= (tiles - 1) >> together; g++) {
             if (note[warp][g] < s_bound || note[warp][g] == ordered(-kInf)) continue;
-            for (int tile = g << together; tile < min(tiles, (g + 1) << together); tile++)
-#pragma unroll 1
-                for (int vi = v0 + tile * kTileVecs + tid; vi < min(v1, v0 + (tile + 1) * kTileVecs); vi += kThreads) {
+            for (int tile = g << together; tile < min(tiles, (g + 1) << together); tile++) {
+                fetch(tile);
+                uint32_t hit = 0;      // 128-bit words with an element that reaches the bound
+#pragma unroll
+                for (int u = 0; u < kVecs; u++)
+                    hit |= W::any_reaches(W::larger(W::larger(next[u].x, next[u].y), W::larger(next[u].z, next[u].w)), bound_word) ? 1u << u : 0u;
+                for (; hit; hit &= hit - 1) {
+                    const int vi = first_of(tile) + lane + (__ffs(hit) - 1) * 32, at = head + vi * kPer;
+                    if (vi >= v1) continue;      // (the fill behind the part's last word reaches a bound of -inf)
                     const uint4 r = __ldg(xv + vi);
-                    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        if (W::any_reaches(w[j], bound_word)) {
-#pragma unroll
-                            for (int e = 0; e < W::kElems; e++) collect(W::get(w[j], e), head + vi * kPer + j * W::kElems + e, bound);
-                        }
+                    for (uint32_t m = W::reaching(r, bound_word); m; m &= m - 1) {
+                        const int e = __ffs(m) - 1;
+                        collect(load_logit(x + at + e), at + e, bound);
+                    }
                 }
+            }
         }
         collect(extra_x, extra_at, bound);
         __syncthreads();
@@ -434,64 +520,64 @@ logprobs_kernel(LogprobArgs a) {
         if (count <= kCandidates) {
             // an element's place is the number of better ones
             for (int q = tid; q < count; q += kThreads) {
-                const float v = c_val[q];
-                const int i = c_idx[q];
-                int place = 0;
-#pragma unroll 4
-                for (int o = 0; o < count; o++) place += better(c_val[o], c_idx[o], v, i);
-                if (place < n) m_val[place] = v, m_idx[place] = i;
+                const uint64_t k = found[q];
+                const int place = larger_than(found, count, k);
+                if (place < n) best[place] = k;
             }
         } else {
             TopList top;
             for (int vi = v0 + warp * 32; vi < v1; vi += kThreads)
                 for (int e = 0; e < kPer; e++) {
                     const int at = head + min(vi + lane, v1 - 1) * kPer + e;
-                    top.offer(vi + lane < v1 ? load_logit(x + at) : -kInf, at, bound, n, lane);
+                    const float v = vi + lane < v1 ? load_logit(x + at) : -kInf;
+                    top.offer(v >= bound && v > -kInf ? key_of(v, at) : 0, n, lane);
                 }
-            top.offer(extra_x, extra_at, bound, n, lane);
-            l_val[warp][lane] = top.v, l_idx[warp][lane] = top.i;
+            top.offer(extra_x >= bound && extra_x > -kInf ? key_of(extra_x, extra_at) : 0, n, lane);
+            // (in the place of the candidates; kWarps lists of 32)
+            found[tid] = top.k;
             __syncthreads();
-            for (int q = tid; q < kWarps * n; q += kThreads) {
-                const int place = merged_place(l_val, l_idx, kWarps, n, q / n, q % n);
-                if (place < n) m_val[place] = l_val[q / n][q % n], m_idx[place] = l_idx[q / n][q % n];
+            if (lane < n) {
+                int place = 0;
+                for (int o = 0; o < kWarps; o++)
+                    for (int q = 0; q < n; q++) place += found[o * 32 + q] > top.k;
+                if (top.k != 0 && place < n) best[place] = top.k;
             }
         }
-    }
-    if (parts > 1) {
-        cluster.sync();
-        if (part == 0) {
-            for (int q = tid; q < parts * n; q += kThreads) {
-                l_val[q / n][q % n] = cluster.map_shared_rank(m_val, q / n)[q % n];
-                l_idx[q / n][q % n] = cluster.map_shared_rank(m_idx, q / n)[q % n];
-            }
-            if (warp == kWarps - 1) {
-                Stats one;
-                int sum = 0;
-                if (lane < parts) {
-                    const float* const o = cluster.map_shared_rank(c_stat, lane);
-                    one.m = o[0], one.s = o[1], one.t = o[2];
-                    sum = *cluster.map_shared_rank(&c_rank, lane);
-                }
-                one.join_warp();
-                sum = __reduce_add_sync(0xffffffffu, sum);
-                if (lane == 0) p_stat[0][0] = one.m, p_stat[0][1] = one.s, p_stat[0][2] = one.t, p_rank[0] = sum;
-            }
-        }
-        cluster.sync();       // the others' shared memory has been read
-        if (part != 0) return;
-        for (int q = tid; q < parts * n; q += kThreads) {
-            const int place = merged_place(l_val, l_idx, parts, n, q / n, q % n);
-            if (place < n) m_val[place] = l_val[q / n][q % n], m_idx[place] = l_idx[q / n][q % n];
-        }
-    } else if (tid == kThreads - 32) {
-        p_stat[0][0] = c_stat[0], p_stat[0][1] = c_stat[1], p_stat[0][2] = c_stat[2];
-        p_rank[0] = c_rank;
     }
     __syncthreads();
+    if (parts > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");      // the first CTA runs and has its barrier
+    if (warp != 0) return;
+    if (parts > 1) {
+        const uint32_t bar = shared_addr(&arrived);
+        if (part != 0) {
+            const uint32_t to = in_first_cta(bar);
+            if (lane < 4) send(in_first_cta(shared_addr(&c_all[part][lane])), c_all[part][lane], to);
+            if (lane < n) {
+                const uint32_t at = in_first_cta(shared_addr(&lists[part][lane]));
+                send(at, (uint32_t)best[lane], to);
+                send(at + 4, (uint32_t)(best[lane] >> 32), to);
+            }
+            return;
+        }
+        lists[0][lane] = best[lane];
+        if (!__all_sync(0xffffffffu, wait_for(bar, 0))) {
+            if (lane == 0) atomicExch(a.err, 3);
+            return;
+        }
+    }
+    uint64_t mine = best[lane];
+    if (parts > 1 && n > 0) mine = merge_lists(lists, parts, n, lane, found, best);
+    Stats all;
+    int rank = 0;
+    if (lane < parts) {
+        all.m = __uint_as_float(c_all[lane][0]), all.s = __uint_as_float(c_all[lane][1]), all.t = __uint_as_float(c_all[lane][2]);
+        rank = (int)c_all[lane][3];
+    }
+    all.join_warp();
+    rank = __reduce_add_sync(0xffffffffu, rank);
 
     // ---- results ------------------------------------------------------------------------------------
-    if (warp != 0) return;
-    const float m = p_stat[0][0], total = p_stat[0][1], t = p_stat[0][2];
+    const float m = all.m, total = all.s, t = all.t;
     const bool broken = total != total, empty = !broken && m == -kInf;
     const float log_s = empty ? 0.f : logf(total);
     const float nan = __int_as_float(0x7fffffff);
@@ -501,13 +587,14 @@ logprobs_kernel(LogprobArgs a) {
         if (a.logprob) a.logprob[row] = wrong ? nan : asked ? prob(x_id) : 0.f;
         const float h = log_s - t / total;
         if (a.entropy) a.entropy[row] = broken ? nan : empty || h < 0.f ? 0.f : h;
-        if (a.rank) a.rank[row] = asked ? p_rank[0] : -1;
+        if (a.rank) a.rank[row] = asked ? rank : -1;
     }
     if (n > 0) {
-        float v = lane < n ? m_val[lane] : -kInf;
-        int i = lane < n ? m_idx[lane] : INT_MAX;
+        const bool real = lane < n && mine != 0;
+        const float v = real ? key_value(mine) : -kInf;
+        int i = real ? key_index(mine) : INT_MAX;
         // fewer than n elements above -inf: the lowest indices of the others follow.  They are within the first 64.
-        const int have = __popc(__ballot_sync(0xffffffffu, lane < n && i != INT_MAX));
+        const int have = __popc(__ballot_sync(0xffffffffu, real));
         int filled = have;
         for (int base = 0; base < a.vocab && filled < n; base += 32) {
             const int at = base + lane;
@@ -526,16 +613,17 @@ logprobs_kernel(LogprobArgs a) {
 
 template <typename T>
 cudaError_t launch(const LogprobArgs& a, int rows, int parts, cudaStream_t s) {
-    static PerDeviceOnce once;
+    static PerDeviceOnce once_large;
+    cudaError_t e;
     if (parts > 8) {
         int dev = 0;
-        cudaError_t e = cudaGetDevice(&dev);
+        e = cudaGetDevice(&dev);
         if (e != cudaSuccess) return e;
         const uint64_t bit = 1ull << (dev & 63);
-        if (!(once.mask.load(std::memory_order_acquire) & bit)) {
+        if (!(once_large.mask.load(std::memory_order_acquire) & bit)) {
             e = cudaFuncSetAttribute(logprobs_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
             if (e != cudaSuccess) return e;
-            once.mask.fetch_or(bit, std::memory_order_release);
+            once_large.mask.fetch_or(bit, std::memory_order_release);
         }
     }
     cudaLaunchConfig_t cfg{};
@@ -548,19 +636,20 @@ cudaError_t launch(const LogprobArgs& a, int rows, int parts, cudaStream_t s) {
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = parts > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, a);
+    return cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, a, parts);
 }
 
 }  // namespace
 
 int launch_logprobs(const void* logits, int dtype, int rows, int vocab, long long stride, const void* ids, int ids_dtype, int top_n,
                     float* logprob, float* entropy, int32_t* rank, int32_t* top_ids, float* top_logprobs, int sm_count,
-                    int32_t* bad_flag, const Ctx& c) {
-    LogprobArgs a{logits, stride, vocab, ids, ids_dtype, top_n, logprob, entropy, rank, top_ids, top_logprobs, bad_flag};
-    // CTAs per row: as many as keep every SM at four, each with a tile of its own at least
+                    int32_t* bad_flag, int32_t* err, const Ctx& c) {
+    LogprobArgs a{logits, stride, vocab, ids, ids_dtype, top_n, logprob, entropy, rank, top_ids, top_logprobs, bad_flag, err};
+    // CTAs per row: as many as keep every SM at four (clusters of more than eight do not pack that well: up to one per SM), each with
+    // two tiles of its own at least
+    const long long tiles = ((long long)vocab * (dtype == 0 ? 2 : 4) + kTileBytes - 1) / kTileBytes;
     int parts = 1;
-    const int tile = kThreads * kVecs * (dtype == 0 ? 8 : 4);
-    while (parts < kMaxCluster && (long long)rows * parts * 2 <= 4ll * sm_count && vocab / (parts * 2) >= tile) parts *= 2;
+    while (parts < kMaxCluster && (long long)rows * (parts + 1) <= (parts < 8 ? 4 * sm_count : sm_count) && tiles >= 2 * (parts + 1)) parts++;
     c.begin(K_LOGPROBS);
     const cudaError_t e = dtype == 0 ? launch<__nv_bfloat16>(a, rows, parts, c.s) : launch<float>(a, rows, parts, c.s);
     c.end();
