@@ -7,6 +7,7 @@
 #include <cuda_fp8.h>
 
 #include "common.cuh"
+#include "umma.cuh"
 
 namespace ftm {
 
@@ -70,5 +71,21 @@ __device__ __forceinline__ void fp8_encode(const float (&f)[U][8], uint2 (&codes
 inline bool fp8_rows_aligned(const void* x, int x_dtype, long long stride) {
     return reinterpret_cast<uintptr_t>(x) % 16 == 0 && stride * (x_dtype == 0 ? 2 : 4) % 16 == 0;
 }
+
+// codes [rows, K] row-major, box = one block of 128 k by box_rows rows, 128-byte swizzle
+inline bool fp8_codes_map(CUtensorMap* map, const void* base, int64_t rows, int64_t K, int box_rows) {
+    umma::EncodeTiledFn fn = umma::encode_tiled();
+    if (!fn) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)K};
+    cuuint32_t box[2] = {(cuuint32_t)kFp8Block, (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// fp8_pair.cu: pairs of SMs on tiles of 256 x 256; a negative result is a CUDA error code
+int launch_fp8_pair(const uint8_t* a, const float* a_scale, const uint8_t* w, const float* w_scale, int M, int N, int K, void* out, int out_dtype,
+                    long long ldc, int sm_count, int32_t* err, cudaStream_t s);
 
 }  // namespace ftm

@@ -392,18 +392,6 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     if (split > 1) cluster_join();
 }
 
-// codes [rows, K] row-major, box = one block of 128 k by box_rows rows, 128-byte swizzle
-bool make_codes_map(CUtensorMap* map, const void* base, int64_t rows, int64_t K, int box_rows) {
-    EncodeTiledFn fn = encode_tiled();
-    if (!fn) return false;
-    cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
-    cuuint64_t strides[1] = {(cuuint64_t)K};
-    cuuint32_t box[2] = {(cuuint32_t)kFp8Block, (cuuint32_t)box_rows};
-    cuuint32_t estr[2] = {1, 1};
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int NT, bool FUSED>
 int launch(const uint8_t* codes, const uint8_t* w, Fp8Args a, int sm_count, cudaStream_t s) {
     using S = Shape<NT, FUSED>;
@@ -427,7 +415,7 @@ int launch(const uint8_t* codes, const uint8_t* w, Fp8Args a, int sm_count, cuda
     while (a.stages > 2 && S::bytes(a.stages, split, fused_blocks) > room) a.stages--;
     const size_t smem = S::bytes(a.stages, split, fused_blocks);
     CUtensorMap map_w, map_a;
-    if (!make_codes_map(&map_w, w, a.N, a.K, kRows) || (!FUSED && !make_codes_map(&map_a, codes, a.M, a.K, NT))) return -(int)cudaErrorInvalidValue;
+    if (!fp8_codes_map(&map_w, w, a.N, a.K, kRows) || (!FUSED && !fp8_codes_map(&map_a, codes, a.M, a.K, NT))) return -(int)cudaErrorInvalidValue;
     if (FUSED) map_a = map_w;
     static PerDeviceOnce once;
     cudaError_t e = allow_dyn_smem(once, fp8_umma_kernel<NT, FUSED>, 227 * 1024);
@@ -457,10 +445,14 @@ int launch_fp8_gemm(const uint8_t* a, const float* a_scale, const uint8_t* w, co
     Fp8Args g{};
     g.a_scale = a_scale; g.w_scale = w_scale; g.M = M; g.N = N; g.K = K; g.c = out; g.c_dtype = out_dtype; g.ldc = ldc; g.err = err;
     c.begin(K_FP8_GEMM);
-    const int n = M <= 16   ? launch<16, false>(a, w, g, sm_count, c.s)
-                  : M <= 32 ? launch<32, false>(a, w, g, sm_count, c.s)
-                  : M <= 64 ? launch<64, false>(a, w, g, sm_count, c.s)
-                            : launch<128, false>(a, w, g, sm_count, c.s);
+    int n;
+    if (M > 128)
+        n = launch_fp8_pair(a, a_scale, w, w_scale, M, N, K, out, out_dtype, ldc, sm_count, err, c.s);
+    else
+        n = M <= 16   ? launch<16, false>(a, w, g, sm_count, c.s)
+            : M <= 32 ? launch<32, false>(a, w, g, sm_count, c.s)
+            : M <= 64 ? launch<64, false>(a, w, g, sm_count, c.s)
+                      : launch<128, false>(a, w, g, sm_count, c.s);
     c.end();
     return n;
 }
