@@ -141,6 +141,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         if (lane == 0) *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    pdl_wait();      // (no tensor memory is held while the kernel before may still want some)
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(s_tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -150,6 +151,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // both CTAs run and have their barriers
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    pdl_launch_dependents();
     const uint32_t tmem_base = *s_tmem;
     const int first = blockIdx.x / 2, step = gridDim.x / 2;
 
@@ -219,7 +221,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                     w[q][0] = kb < a.blocks ? __ldg(sw + kb) : 0.f;
                     w[q][1] = kb < a.blocks && second ? __ldg(sw + a.blocks + kb) : 0.f;
 #pragma unroll
-                    for (int j = 0; j < 4; j++) v[q][j] = kb < a.blocks && t0 + 32 * j < a.M ? __ldg(a.a_scale + (size_t)kb * a.M + t0 + 32 * j) : 0.f;
+                    for (int j = 0; j < 4; j++) v[q][j] = kb < a.blocks && t0 + 32 * j < a.M ? __ldcg(a.a_scale + (size_t)kb * a.M + t0 + 32 * j) : 0.f;
                 }
             };
             ask(0, now, now_w);
@@ -253,28 +255,29 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
         const uint32_t release[2] = {in_first_cta(ACC_EMPTY(0)), in_first_cta(ACC_EMPTY(1))};
         int p = 0;
         uint32_t p_round = 0;
-        bool ok = true, seen = false;
+        bool ok = true;
         for (int tile = first; tile < a.tiles && ok; tile += step) {
             const int t0 = tile % a.m_tiles * kM + rank * 128 + quarter * 32, n0 = tile / a.m_tiles * kN + half * 128;
             float acc[128];
 #pragma unroll
             for (int j = 0; j < 128; j++) acc[j] = 0.f;
+            // 32 columns at a time: one of the two warps of an SM's quarter loads while the other adds (a second buffer and loads ahead
+            // of the sums, 64 columns, two sums per instruction, sixteen warps of 64 columns and giving the accumulator back before
+            // the last sums were all slower: 262, 424, 305, 275 and 254 us against 243 at 8192 x 8192 x 4096).
             for (int kb = 0; kb < a.blocks; kb++) {
-                if (!seen) ok = mbar_wait_warp(ACC_FULL(p), p_round, s_abort, a.err);
+                ok = mbar_wait_warp(ACC_FULL(p), p_round, s_abort, a.err);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const bool next_full = mbar_test_wait(ACC_FULL(p ^ 1), p_round ^ p);      // (the round of the other accumulator)
-                float d[2][32];
-                tmem_ld32(taddr + p * kN, d[0]);
                 const float scale = slots[p * 130 + quarter * 32 + lane] * slots[p * 130 + 128 + half];
+                float d[32];
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
+                    tmem_ld32(taddr + p * kN + c * 32, d);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 32; j++) asm volatile("" : "+f"(d[c & 1][j]));      // not read in front of the wait
-                    if (c < 3) tmem_ld32(taddr + p * kN + (c + 1) * 32, d[(c + 1) & 1]);
+                    for (int j = 0; j < 32; j++) asm volatile("" : "+f"(d[j]));      // not read in front of the wait
 #pragma unroll
-                    for (int j = 0; j < 32; j++) acc[c * 32 + j] = fmaf(d[c & 1][j], scale, acc[c * 32 + j]);
+                    for (int j = 0; j < 32; j++) acc[c * 32 + j] = fmaf(d[j], scale, acc[c * 32 + j]);
                 }
                 // (relaxed: what it orders is in tensor memory; a release at cluster scope takes some hundred cycles)
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -284,7 +287,6 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
                     mbar_arrive(SLOT_EMPTY(p));
                 }
                 if (++p == 2) p = 0, p_round ^= 1;
-                seen = __all_sync(0xffffffffu, next_full);
             }
             if (!ok) break;
             if (t0 >= a.M || n0 >= a.N) continue;
@@ -362,8 +364,7 @@ int launch_fp8_pair(const uint8_t* a, const float* a_scale, const uint8_t* w, co
     static PerDeviceOnce once;
     cudaError_t e = allow_dyn_smem(once, fp8_pair_kernel, kSmem);
     if (e != cudaSuccess) return -(int)e;
-    fp8_pair_kernel<<<2 * max(1, min(g.tiles, sm_count / 2)), kThreads, kSmem, s>>>(map_a, map_w, map_c, g);
-    e = cudaGetLastError();
+    e = launch_pdl(fp8_pair_kernel, dim3(2 * max(1, min(g.tiles, sm_count / 2))), dim3(kThreads), kSmem, s, map_a, map_w, map_c, g);
     return e == cudaSuccess ? 1 : -(int)e;
 }
 

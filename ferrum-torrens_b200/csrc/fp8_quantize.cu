@@ -14,7 +14,9 @@ constexpr int kAtOnce = 2;      // blocks a group of lanes holds at a time
 
 template <typename T>
 __global__ void __launch_bounds__(256)
-fp8_quantize_kernel(const T* __restrict__ x, long long stride, int rows, int K, bool vec, uint8_t* __restrict__ q, float* __restrict__ scale) {
+fp8_quantize_kernel(const T* x, long long stride, int rows, int K, bool vec, uint8_t* q, float* scale) {
+    pdl_launch_dependents();
+    pdl_wait();
     const int lane = threadIdx.x % 32, blocks = (K + kFp8Block - 1) / kFp8Block;
     const long long row = (long long)blockIdx.x * 8 + threadIdx.x / 32;
     if (row >= rows) return;
@@ -43,12 +45,11 @@ int launch_fp8_quantize(const void* x, int x_dtype, int rows, int K, long long s
     const bool vec = fp8_rows_aligned(x, x_dtype, stride);
     const dim3 grid(((unsigned)rows + 7) / 8, min((blocks + 2 * kAtOnce - 1) / (2 * kAtOnce), 65535));
     c.begin(K_FP8_QUANTIZE);
-    if (x_dtype == 0)
-        fp8_quantize_kernel<<<grid, 256, 0, c.s>>>((const __nv_bfloat16*)x, stride, rows, K, vec, q, scale);
-    else
-        fp8_quantize_kernel<<<grid, 256, 0, c.s>>>((const float*)x, stride, rows, K, vec, q, scale);
+    const cudaError_t e =
+        x_dtype == 0 ? launch_pdl(fp8_quantize_kernel<__nv_bfloat16>, grid, dim3(256), 0, c.s, (const __nv_bfloat16*)x, stride, rows, K, vec, q, scale)
+                     : launch_pdl(fp8_quantize_kernel<float>, grid, dim3(256), 0, c.s, (const float*)x, stride, rows, K, vec, q, scale);
     c.end();
-    return 1;
+    return e == cudaSuccess ? 1 : -(int)e;
 }
 
 }  // namespace ftm

@@ -166,10 +166,12 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         __syncwarp();
+        pdl_wait();
         if (elect_one())
             for (int i = 0; i < early; i++) load(i, first, kb0 + i);
         __syncwarp();
     }
+    if (warp != 0) pdl_wait();      // (no tensor memory is held while the kernel before may still want some)
     if (warp == 2) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)), "n"(S::kTmem) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -214,6 +216,7 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     // Two barriers of the cluster.  The first: every CTA runs and has its barriers before another one reaches into its shared
     // memory (waited for before the first sums are sent).  The second: none leaves while another may still reach into it.
     if (split > 1) cluster_arrive();
+    pdl_launch_dependents();
     const uint32_t tmem_base = *s_tmem;
     bool joined = split == 1, left = split == 1;      // this thread has waited for the first, has arrived at the second
 
@@ -272,7 +275,7 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
                     for (int j = 0; j < kPer; j++) {
                         const int col = lane + 32 * j, t = t0 + col;
                         float s = 0.f;
-                        if (i < nkb && col < NT && t < a.M) s = FUSED ? row_scales[i * NT + col] : a.a_scale[(size_t)(kb0 + i) * a.M + t];
+                        if (i < nkb && col < NT && t < a.M) s = FUSED ? row_scales[i * NT + col] : __ldcg(a.a_scale + (size_t)(kb0 + i) * a.M + t);
                         v[q][j] = s * ws;
                     }
                 }
@@ -425,12 +428,14 @@ int launch(const uint8_t* codes, const uint8_t* w, Fp8Args a, int sm_count, cuda
     cfg.blockDim = dim3(S::kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = split;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = split;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = split > 1 ? 1 : 0;
+    cfg.numAttrs = split > 1 ? 2 : 1;
     e = cudaLaunchKernelEx(&cfg, fp8_umma_kernel<NT, FUSED>, map_w, map_a, a, split);
     return e == cudaSuccess ? 1 : -(int)e;
 }
