@@ -1300,7 +1300,7 @@ FTM_API int ftm_fp8_quantize(ftm_handle* h, const void* x, int x_dtype, int32_t 
     int rc = check_fp8_rows(h, "fp8 quantize", x, x_dtype, rows, k, x_stride);
     if (rc == FTM_OK) rc = check_fp8_codes(h, "fp8 quantize", q_e4m3, scale);
     if (rc != FTM_OK) return rc;
-    return count_launches(h, launch_fp8_quantize(x, x_dtype, rows, k, x_stride, (uint8_t*)q_e4m3, scale, h->ctx(pick(h, stream))), "fp8 quantize");
+    return count_launches(h, launch_fp8_quantize(x, x_dtype, rows, k, x_stride, (uint8_t*)q_e4m3, scale, h->sm_count, h->ctx(pick(h, stream))), "fp8 quantize");
 }
 
 FTM_API int ftm_fp8_gemm(ftm_handle* h, const void* a_e4m3, const float* a_scale, const void* w_e4m3, const float* w_scale, int32_t m, int32_t n,
@@ -1333,7 +1333,7 @@ FTM_API int ftm_fp8_linear(ftm_handle* h, const void* x, int x_dtype, int64_t x_
     if (!q_scratch || !scale_scratch) return fail(h, FTM_ERR_BAD, "moe: fp8 linear: %d rows of %d need scratch for their codes and scales", m, k);
     rc = check_fp8_codes(h, "fp8 linear", q_scratch, scale_scratch);
     if (rc != FTM_OK) return rc;
-    rc = count_launches(h, launch_fp8_quantize(x, x_dtype, m, k, x_stride, (uint8_t*)q_scratch, scale_scratch, ctx), "fp8 quantize");
+    rc = count_launches(h, launch_fp8_quantize(x, x_dtype, m, k, x_stride, (uint8_t*)q_scratch, scale_scratch, h->sm_count, ctx), "fp8 quantize");
     if (rc != FTM_OK) return rc;
     return count_launches(h, launch_fp8_gemm((const uint8_t*)q_scratch, scale_scratch, (const uint8_t*)w_e4m3, w_scale, m, n, k, c, c_dtype, c_stride,
                                              h->sm_count, h->flags + 2, ctx), "fp8 linear");

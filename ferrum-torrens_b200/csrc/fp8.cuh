@@ -15,40 +15,67 @@ constexpr int kFp8Block = 128;                       // k of one scale
 constexpr float kFp8Max = 448.0f;                    // largest e4m3 value
 constexpr float kFp8Least = 0x1.cp-118f;             // 448 * 2^-126: 448 / a0 and a0 / 448 stay normal
 
-// eight elements of a row; elements from `valid` on are zero and not read.  vec: the rows start on 16-byte boundaries.
+// Eight elements of a row as they are in memory.
 template <typename T>
-__device__ __forceinline__ void fp8_load8(const T* p, bool vec, int valid, float (&f)[8]) {
-    if (vec && valid >= 8) {
-        if constexpr (sizeof(T) == 2) {
-            const uint4 v = *reinterpret_cast<const uint4*>(p);
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float2 q = bf16x2_to_f32(w[j]);
-                f[2 * j] = q.x, f[2 * j + 1] = q.y;
-            }
-        } else {
-            const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-            f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; j++) f[j] = j < valid ? (float)p[j] : 0.f;
+struct Fp8Eight;
+template <>
+struct Fp8Eight<__nv_bfloat16> {
+    uint32_t w[4];
+    __device__ __forceinline__ void load(const __nv_bfloat16* p) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
     }
+    __device__ __forceinline__ void gather(const __nv_bfloat16* p, int valid) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const __nv_bfloat162 v = __halves2bfloat162(2 * j < valid ? p[2 * j] : __float2bfloat16(0.f), 2 * j + 1 < valid ? p[2 * j + 1] : __float2bfloat16(0.f));
+            w[j] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+    }
+    // the largest magnitude (a NaN does not count), two at a time
+    __device__ __forceinline__ float most() const {
+        auto mag = [&](int j) { return __habs2(*reinterpret_cast<const __nv_bfloat162*>(w + j)); };
+        const __nv_bfloat162 m = __hmax2(__hmax2(mag(0), mag(1)), __hmax2(mag(2), mag(3)));
+        return fmaxf(__low2float(m), __high2float(m));
+    }
+    __device__ __forceinline__ float2 two(int j) const { return bf16x2_to_f32(w[j]); }
+};
+template <>
+struct Fp8Eight<float> {
+    float f[8];
+    __device__ __forceinline__ void load(const float* p) {
+        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+        f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+    }
+    __device__ __forceinline__ void gather(const float* p, int valid) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) f[j] = j < valid ? p[j] : 0.f;
+    }
+    __device__ __forceinline__ float most() const {
+        float m = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf(f[j]));
+        return m;
+    }
+    __device__ __forceinline__ float2 two(int j) const { return make_float2(f[2 * j], f[2 * j + 1]); }
+};
+// elements from `valid` on are zero and not read.  vec: the rows start on 16-byte boundaries.
+template <typename T>
+__device__ __forceinline__ void fp8_load8(const T* p, bool vec, int valid, Fp8Eight<T>& f) {
+    if (vec && valid >= 8) f.load(p);
+    else f.gather(p, valid);
 }
 
 // Codes and scales of U blocks at once, each held by sixteen neighbouring lanes, eight elements per lane.  Rounds to nearest even,
 // saturates; a NaN stays one and does not count as a magnitude.  The 2 U quotients of a group are one division, of lane j < 2 U.
-template <int U>
-__device__ __forceinline__ void fp8_encode(const float (&f)[U][8], uint2 (&codes)[U], float (&scale)[U]) {
+template <int U, typename T>
+__device__ __forceinline__ void fp8_encode(const Fp8Eight<T> (&f)[U], uint2 (&codes)[U], float (&scale)[U]) {
     static_assert(U <= 8, "a lane for each quotient");
     const int lane = threadIdx.x % 16, group = threadIdx.x % 32 - lane;
     float num = 1.f, den = 1.f;
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        float most = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; j++) most = fmaxf(most, fabsf(f[u][j]));
+        float most = f[u].most();
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
         most = fmaxf(most, kFp8Least);
@@ -62,8 +89,10 @@ __device__ __forceinline__ void fp8_encode(const float (&f)[U][8], uint2 (&codes
         scale[u] = __shfl_sync(0xffffffffu, quotient, group + 2 * u + 1);
         uint32_t c[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            c[j] = __nv_cvt_float2_to_fp8x2(make_float2(f[u][2 * j] * inv, f[u][2 * j + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+        for (int j = 0; j < 4; j++) {
+            const float2 v = f[u].two(j);
+            c[j] = __nv_cvt_float2_to_fp8x2(make_float2(v.x * inv, v.y * inv), __NV_SATFINITE, __NV_E4M3);
+        }
         codes[u] = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
     }
 }

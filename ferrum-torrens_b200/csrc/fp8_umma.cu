@@ -17,6 +17,8 @@
 // FUSED (at most 16 tokens): the rows are still bf16 or f32.  The epilogue warps first quantise the CTA's share of them
 // into the swizzled operand layout, while the first weight boxes are on their way; they stay there for all tiles.
 // Every wait is bounded; a wait that gives up raises the error flag and the CTA drains.
+#include <type_traits>
+
 #include "fp8.cuh"
 #include "kernels.cuh"
 #include "umma.cuh"
@@ -183,28 +185,30 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
         constexpr int kGroups = 2 * (S::kEpi + S::kHelp), kAtOnce = 4;
         const int piece = lane % 16, units = nkb * a.M;
         const uint32_t by_m = 65536u / a.M + 1;      // (w * by_m) >> 16 = w / M for w < 65536 / M
-        for (int w0 = etid / 32 * 2; w0 < units; w0 += kGroups * kAtOnce) {
-            float f[kAtOnce][8], sc[kAtOnce];
-            uint2 q[kAtOnce];
-            int at[kAtOnce], row[kAtOnce];
+        auto quantise = [&](auto* x) {
+            using T = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
+            for (int w0 = etid / 32 * 2; w0 < units; w0 += kGroups * kAtOnce) {
+                Fp8Eight<T> f[kAtOnce];
+                float sc[kAtOnce];
+                uint2 q[kAtOnce];
+                int at[kAtOnce], row[kAtOnce];
 #pragma unroll
-            for (int u = 0; u < kAtOnce; u++) {
-                const int w = w0 + lane / 16 + u * kGroups, i = (w * by_m) >> 16, r = w - i * a.M, k = (kb0 + i) * kFp8Block + piece * 8;
-                const int valid = w < units ? a.K - k : 0;
-                at[u] = i, row[u] = r;
-                if (a.x_dtype == 0)
-                    fp8_load8(reinterpret_cast<const __nv_bfloat16*>(a.x) + r * a.x_stride + k, a.x_vec, valid, f[u]);
-                else
-                    fp8_load8(reinterpret_cast<const float*>(a.x) + r * a.x_stride + k, a.x_vec, valid, f[u]);
-            }
-            fp8_encode(f, q, sc);
+                for (int u = 0; u < kAtOnce; u++) {
+                    const int w = w0 + lane / 16 + u * kGroups, i = (w * by_m) >> 16, r = w - i * a.M, k = (kb0 + i) * kFp8Block + piece * 8;
+                    at[u] = i, row[u] = r;
+                    fp8_load8(x + r * a.x_stride + k, a.x_vec, w < units ? a.K - k : 0, f[u]);
+                }
+                fp8_encode(f, q, sc);
 #pragma unroll
-            for (int u = 0; u < kAtOnce; u++) {
-                if (w0 + lane / 16 + u * kGroups >= units) continue;
-                *reinterpret_cast<uint2*>(codes + at[u] * S::kABytes + row[u] * 128 + (((piece >> 1) ^ (row[u] & 7)) << 4) + (piece & 1) * 8) = q[u];
-                if (piece == 0) row_scales[at[u] * NT + row[u]] = sc[u];
+                for (int u = 0; u < kAtOnce; u++) {
+                    if (w0 + lane / 16 + u * kGroups >= units) continue;
+                    *reinterpret_cast<uint2*>(codes + at[u] * S::kABytes + row[u] * 128 + (((piece >> 1) ^ (row[u] & 7)) << 4) + (piece & 1) * 8) = q[u];
+                    if (piece == 0) row_scales[at[u] * NT + row[u]] = sc[u];
+                }
             }
-        }
+        };
+        if (a.x_dtype == 0) quantise(reinterpret_cast<const __nv_bfloat16*>(a.x));
+        else quantise(reinterpret_cast<const float*>(a.x));
         // rows past M are zero
         for (int w = etid; w < nkb * (NT * 8); w += 32 * (S::kEpi + S::kHelp))
             if (w / 8 % NT >= a.M) *reinterpret_cast<uint4*>(codes + w * 16) = make_uint4(0, 0, 0, 0);

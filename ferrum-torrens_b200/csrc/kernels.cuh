@@ -258,7 +258,7 @@ int launch_dense_gemv(const void* a, int a_dtype, const uint32_t* packed, const 
 
 // fp8_quantize.cu, fp8_umma.cu: block-scaled 8-bit products and the quantisation of their activations; a negative result is a
 // CUDA error code
-int launch_fp8_quantize(const void* x, int x_dtype, int rows, int K, long long stride, uint8_t* q, float* scale, const Ctx& c);
+int launch_fp8_quantize(const void* x, int x_dtype, int rows, int K, long long stride, uint8_t* q, float* scale, int sm_count, const Ctx& c);
 int launch_fp8_gemm(const uint8_t* a, const float* a_scale, const uint8_t* w, const float* w_scale, int M, int N, int K, void* out,
                     int out_dtype, long long ldc, int sm_count, int32_t* err, const Ctx& c);
 // quantisation and product in one kernel
