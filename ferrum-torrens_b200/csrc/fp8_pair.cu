@@ -102,13 +102,14 @@ __device__ __forceinline__ void send_out(const PairArgs& a, const CUtensorMap* m
     }
     // rows that are less aligned: lanes side by side along a row, as many bytes each as the alignment allows
     __syncwarp();
-    const int log_piece = a.c_align == 8 ? 3 : a.c_align == 4 ? 2 : 1, per_row = 256 >> log_piece;
-    for (int i = lane; i < 32 * per_row; i += 32) {
-        const int row = i / per_row, byte = (i - row * per_row) << log_piece, col = n0 + byte / elem;
+    const int log_piece = a.c_align == 8 ? 3 : a.c_align == 4 ? 2 : 1, log_elem = elem == 2 ? 1 : 2, piece = 1 << log_piece;
+#pragma unroll 4
+    for (int i = 0; i < 256 >> log_piece; i++) {      // 32 pieces each time
+        const int at = (i * 32 << log_piece) + (lane << log_piece), row = at >> 8, byte = at & 255, col = n0 + (byte >> log_elem);
         if (t0 + row >= a.M || col >= a.N) continue;
         const uint8_t* const src = from + (byte >> 7) * 4096 + row * 128 + ((((byte >> 4) & 7) ^ (row & 7)) << 4) + (byte & 15);
-        uint8_t* const dst = reinterpret_cast<uint8_t*>(a.c) + ((t0 + row) * a.ldc + col) * elem;
-        const int bytes = min(1 << log_piece, (a.N - col) * elem);
+        uint8_t* const dst = reinterpret_cast<uint8_t*>(a.c) + (((t0 + row) * a.ldc + col) << log_elem);
+        const int bytes = min(piece, (a.N - col) << log_elem);
         if (bytes == 8) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(src);
         else if (bytes == 4) *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
         else

@@ -17,6 +17,7 @@
 // FUSED (at most 16 tokens): the rows are still bf16 or f32.  The epilogue warps first quantise the CTA's share of them
 // into the swizzled operand layout, while the first weight boxes are on their way; they stay there for all tiles.
 // Every wait is bounded; a wait that gives up raises the error flag and the CTA drains.
+#include <atomic>
 #include <type_traits>
 
 #include "fp8.cuh"
@@ -53,9 +54,11 @@ __device__ __forceinline__ uint32_t map_shared_to(uint32_t addr, uint32_t rank) 
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
-// a store into another CTA's shared memory that counts its bytes on a barrier there: no fence, and who waits sees the value
-__device__ __forceinline__ void remote_store(uint32_t addr, float v, uint32_t bar) {
-    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(addr), "r"(__float_as_uint(v)), "r"(bar) : "memory");
+// a store into another CTA's shared memory that counts its bytes on a barrier there: no fence, and who waits sees the values
+__device__ __forceinline__ void remote_store(uint32_t addr, const float* v, uint32_t bar) {
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(addr), "r"(__float_as_uint(v[0])),
+                 "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])), "r"(bar)
+                 : "memory");
 }
 __device__ __forceinline__ void remote_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -117,8 +120,10 @@ struct Shape {
     static constexpr int kPerSm = NT <= 32 ? 2 : 1;              // CTAs of an SM
     static constexpr size_t kSmem = kPerSm == 2 ? 113 * 1024 : 227 * 1024;
     static constexpr int kStage = kWBytes + (FUSED ? 0 : kABytes);
-    // after the ring: sums from the cluster's CTAs [ranks][NT / ranks][128], slots of scales, FUSED: codes and scales of the rows
-    static __host__ __device__ int sum_floats(int split) { return (NT + split - 1) / split * split * kRows; }
+    // after the ring: sums from the cluster's CTAs [ranks][groups of tokens][128] x 4, slots of scales, FUSED: codes and scales of the rows
+    // groups of four tokens that one CTA of a cluster finishes, and what they take of its shared memory
+    static __host__ __device__ int share(int split) { return (NT / 4 + split - 1) / split; }
+    static __host__ __device__ int sum_floats(int split) { return share(split) * split * 4 * kRows; }
     static size_t bytes(int stages, int split, int fused_blocks) {
         return 1024 + (size_t)stages * kStage + (FUSED ? (size_t)fused_blocks * (kABytes + NT * 4) : 0) + (split > 1 ? (size_t)sum_floats(split) * 4 : 0) +
                kAcc * NT * 4 + kBarBytes;
@@ -355,21 +360,22 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
                 }
                 continue;
             }
-            // the cluster's sums: token j belongs to the CTA j / share
-            const int share = (NT + split - 1) / split, mine = min(min(share, NT - rank * share), a.M - t0 - rank * share);
+            // the cluster's sums: the group of tokens 4 g .. 4 g + 3 belongs to the CTA g / share.  A lane is a weight row, so its four
+            // sums of a group are one store of 16 bytes, beside its neighbours'.
+            const int share = S::share(split), groups = (min(NT, a.M - t0) + 3) / 4, mine = min(share, groups - rank * share);
             const bool last = tile + step >= a.tiles;
-            if (etid == 0 && mine > 0) mbar_expect_tx(SUM_FULL, split * mine * kRows * 4);
+            if (etid == 0 && mine > 0) mbar_expect_tx(SUM_FULL, split * mine * kRows * 16);
             if (!joined) cluster_join(), joined = true;
             if (done > 0) ok = __all_sync(0xffffffffu, cluster_wait(SUM_FREE, (done - 1) & 1, s_abort, a.err));
             if (!ok) break;
-            const uint32_t my_sums = smem_u32(sums + rank * share * kRows + row);
+            const uint32_t my_sums = smem_u32(sums + (rank * share * kRows + row) * 4);
             uint32_t to_sums = 0, to_bar = 0;
-            int to = col0 / share, in_share = col0 - to * share;
+            int to = col0 / 4 / share, in_share = col0 / 4 - to * share;
 #pragma unroll
-            for (int j = 0; j < S::kCols; j++) {
-                if (t0 + col0 + j >= a.M) break;
+            for (int j = 0; j < S::kCols / 4; j++) {
+                if (col0 / 4 + j >= groups) break;
                 if (j == 0 || in_share == 0) to_sums = map_shared_to(my_sums, to), to_bar = map_shared_to(SUM_FULL, to);
-                remote_store(to_sums + in_share * kRows * 4, acc[j], to_bar);
+                remote_store(to_sums + in_share * kRows * 16, acc + 4 * j, to_bar);
                 if (++in_share == share) in_share = 0, to++;
             }
             __syncwarp();
@@ -378,13 +384,20 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
                 ok = __all_sync(0xffffffffu, cluster_wait(SUM_FULL, got++ & 1, s_abort, a.err));
                 if (!ok) break;
                 for (int q = etid; q < mine * kRows; q += 32 * S::kEpi) {
-                    const int j = q / kRows, n = q % kRows;
-                    float v[kMaxSplit], sum = 0.f;
+                    const int g = q / kRows, n = q % kRows, t = t0 + (rank * share + g) * 4;
+                    float4 v[kMaxSplit], sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                    for (int r = 0; r < kMaxSplit; r++) v[r] = r < split ? sums[(r * share + j) * kRows + n] : 0.f;
+                    for (int r = 0; r < kMaxSplit; r++)
+                        v[r] = r < split ? reinterpret_cast<const float4*>(sums)[(r * share + g) * kRows + n] : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                    for (int r = 0; r < kMaxSplit; r++) sum += v[r];
-                    if (n0 + n < a.N) store_act(a.c, a.c_dtype, (size_t)(t0 + rank * share + j) * a.ldc + n0 + n, sum);
+                    for (int r = 0; r < kMaxSplit; r++) sum.x += v[r].x, sum.y += v[r].y, sum.z += v[r].z, sum.w += v[r].w;
+                    if (n0 + n < a.N) {
+                        const float out[4] = {sum.x, sum.y, sum.z, sum.w};
+                        const size_t at = (size_t)t * a.ldc + n0 + n;
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            if (t + j < a.M) store_act(a.c, a.c_dtype, at + j * a.ldc, out[j]);
+                    }
                 }
             }
             __syncwarp();
@@ -399,21 +412,61 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     if (split > 1) cluster_join();
 }
 
+// Clusters of q CTAs that the device holds at a time (SMs are grouped, so eights and sevens leave some of them empty)
+template <int NT, bool FUSED>
+int clusters_at_once(int q) {
+    static std::atomic<int> known[64][kMaxSplit + 1];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return 0;
+    int n = known[dev][q].load(std::memory_order_relaxed);
+    if (n) return n;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(q);
+    cfg.blockDim = dim3(Shape<NT, FUSED>::kThreads);
+    cfg.dynamicSmemBytes = Shape<NT, FUSED>::kSmem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = q;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, fp8_umma_kernel<NT, FUSED>, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        n = 1;
+    }
+    known[dev][q].store(max(n, 1), std::memory_order_relaxed);
+    return max(n, 1);
+}
+
+// CTAs that share a tile's blocks, and what a call then waits for, in blocks of one CTA
+struct Plan {
+    int split, cost;
+};
+template <int NT, bool FUSED>
+Plan plan_for(int M, int N, int blocks, int sm_count) {
+    using S = Shape<NT, FUSED>;
+    const long long tiles = (long long)((M + NT - 1) / NT) * ((N + kRows - 1) / kRows);
+    const int join = NT <= 64 ? 6 : 9;      // what joining the sums costs, in blocks (13 or more were slower at 2048 rows, fewer at 8192)
+    Plan best{1, (int)min((tiles + sm_count - 1) / sm_count * blocks, 1ll << 30)};
+    for (int q = 2; q <= kMaxSplit && q <= blocks && tiles * q <= S::kPerSm * sm_count; q++) {
+        if (tiles > clusters_at_once<NT, FUSED>(q)) continue;
+        const int cost = (int)((tiles * q + sm_count - 1) / sm_count) * ((blocks + q - 1) / q) + join;
+        if (cost < best.cost) best = {q, cost};
+    }
+    return best;
+}
+
 template <int NT, bool FUSED>
 int launch(const uint8_t* codes, const uint8_t* w, Fp8Args a, int sm_count, cudaStream_t s) {
     using S = Shape<NT, FUSED>;
     a.blocks = (a.K + kFp8Block - 1) / kFp8Block;
     a.t_tiles = (a.M + NT - 1) / NT;
     a.tiles = a.t_tiles * ((a.N + kRows - 1) / kRows);
-    // Too few tiles to keep every SM loading: the CTAs of a cluster share a tile's blocks.  The busiest SM's blocks are what a call
-    // waits for; joining the sums costs about as much as three blocks.
-    int split = 1;
-    long long best = 0;
-    for (int q = 1; q <= kMaxSplit && q <= a.blocks; q++) {
-        if (q > 1 && (long long)a.tiles * q > (q <= 4 ? S::kPerSm * sm_count : S::kPerSm * sm_count * 7 / 8)) break;     // larger clusters do not fill every SM
-        const long long cost = ((long long)a.tiles * q + sm_count - 1) / sm_count * ((a.blocks + q - 1) / q) + (q > 1 ? 3 : 0);
-        if (q == 1 || cost < best) best = cost, split = q;
-    }
+    static PerDeviceOnce once;
+    cudaError_t e = allow_dyn_smem(once, fp8_umma_kernel<NT, FUSED>, 227 * 1024);
+    if (e != cudaSuccess) return -(int)e;
+    const Plan plan = plan_for<NT, FUSED>(a.M, a.N, a.blocks, sm_count);
+    const int split = plan.split;
     const int fused_blocks = (a.blocks + split - 1) / split;
     // FUSED with many blocks to a CTA: its codes leave room for two boxes beside a second CTA, or the SM is its own
     size_t room = S::kSmem;
@@ -424,9 +477,6 @@ int launch(const uint8_t* codes, const uint8_t* w, Fp8Args a, int sm_count, cuda
     CUtensorMap map_w, map_a;
     if (!fp8_codes_map(&map_w, w, a.N, a.K, kRows) || (!FUSED && !fp8_codes_map(&map_a, codes, a.M, a.K, NT))) return -(int)cudaErrorInvalidValue;
     if (FUSED) map_a = map_w;
-    static PerDeviceOnce once;
-    cudaError_t e = allow_dyn_smem(once, fp8_umma_kernel<NT, FUSED>, 227 * 1024);
-    if (e != cudaSuccess) return -(int)e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(split * max(1, min(a.tiles, S::kPerSm * sm_count / split)));
     cfg.blockDim = dim3(S::kThreads);
@@ -455,7 +505,10 @@ int launch_fp8_gemm(const uint8_t* a, const float* a_scale, const uint8_t* w, co
     g.a_scale = a_scale; g.w_scale = w_scale; g.M = M; g.N = N; g.K = K; g.c = out; g.c_dtype = out_dtype; g.ldc = ldc; g.err = err;
     c.begin(K_FP8_GEMM);
     int n;
-    if (M > 128)
+    // (a pair's block of 256 x 256 takes 0.43 to 0.49 us, one of 128 x 128 here 0.40)
+    const int blocks = (K + kFp8Block - 1) / kFp8Block;
+    const long long pair_tiles = (long long)((M + 255) / 256) * ((N + 255) / 256), pair_cost = (pair_tiles + sm_count / 2 - 1) / max(1, sm_count / 2) * blocks * 9 / 8;
+    if (M > 128 && sm_count > 1 && pair_cost < plan_for<128, false>(M, N, blocks, sm_count).cost)
         n = launch_fp8_pair(a, a_scale, w, w_scale, M, N, K, out, out_dtype, ldc, sm_count, err, c.s);
     else
         n = M <= 16   ? launch<16, false>(a, w, g, sm_count, c.s)
