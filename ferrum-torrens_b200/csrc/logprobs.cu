@@ -9,8 +9,8 @@
 // maximum rises (t gains s * (old - new)); the partial triples are joined over the warp, the CTA and the cluster.
 // Differences are clamped at -1e20: an element of -inf adds e^d = 0 times a finite d; NaN and +inf make s a NaN.
 //
-// Alternatives (n <= 32).  The pass itself only notes the maximum of every warp's part of every tile.  The 256 lanes' maxima,
-// taken together by fours, give 64 values, and the n-th largest of these is a bound: n elements reach it, so what is below
+// Alternatives (n <= 32).  The pass itself only notes the maximum of every warp's part of every tile.  The lanes' maxima, some
+// taken together, give 64 values, and the n-th largest of these is a bound: n elements reach it, so what is below
 // cannot belong to the answer.  The tiles whose maximum reaches it are read again (from L2 mostly), the elements that reach it
 // are collected and placed by counting the better ones.  Where ties make them too many, every warp keeps its n best as
 // a sorted list over its lanes instead.
@@ -27,18 +27,14 @@ namespace ftm {
 
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
 constexpr int kMaxCluster = 16;      // more than 8 CTAs need the opt-in of launch_logprobs
 constexpr int kVecs = 4;             // 128-bit words of a lane per tile
 constexpr int kWarpVecs = 32 * kVecs;        // 128-bit words of a warp per tile
-constexpr int kTileVecs = kWarps * kWarpVecs;
-constexpr int kTileBytes = kTileVecs * 16;   // 16 KiB
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kInf = __builtin_huge_valf();
 constexpr float kFar = -1e20f;       // differences below this have exponential 0; clamped there, sums of them stay finite
 constexpr int kCandidates = 512;
-constexpr int kNotes = 32;           // noted maxima of a warp; longer parts note several tiles together
+constexpr int kNotes = 64;           // noted maxima of a warp; longer parts note several tiles together
 constexpr uint32_t kSpin = 1u << 20; // looks at a barrier before a wait is given up
 
 __device__ __forceinline__ float ex2(float v) {
@@ -170,7 +166,7 @@ struct Stats {
             m = mx;
         }
     }
-    // the elements of one 128-bit vector; s2 and t2 hold sums of even and odd elements until take()
+    // the elements of one 128-bit word; s2 and t2 hold sums of even and odd elements until take()
     template <typename T>
     __device__ __forceinline__ void add(const uint4& v, uint64_t& s2, uint64_t& t2) const {
         const float from = m == -kInf ? 0.f : -m;
@@ -336,11 +332,12 @@ struct LogprobArgs {
     int32_t* err;
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 4)
+template <typename T, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, 32 / kWarps)
 logprobs_kernel(LogprobArgs a, int parts) {
     using W = Word<T>;
     constexpr int kPer = 4 * W::kElems;           // elements of a 128-bit word
+    constexpr int kThreads = kWarps * 32, kTileVecs = kWarps * kWarpVecs;
     const long long row = blockIdx.x / parts;
     const int part = blockIdx.x - (int)row * parts;        // (a cluster is one row's CTAs, in their order)
     const T* const x = reinterpret_cast<const T*>(a.logits) + row * a.stride;
@@ -360,7 +357,7 @@ logprobs_kernel(LogprobArgs a, int parts) {
     // whole 128-bit words of the row, and the elements in front of and behind them
     const int head = min((int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)), a.vocab);
     const int vecs = (a.vocab - head) / kPer, tail = a.vocab - head - vecs * kPer;
-    const int v0 = (int)((long long)vecs * part / parts), v1 = (int)((long long)vecs * (part + 1) / parts);
+    const int each = vecs / parts, more = vecs - each * parts, v0 = part * each + min(part, more), v1 = v0 + each + (part < more);
     const uint4* const xv = reinterpret_cast<const uint4*>(x + head);
     // tiles of this CTA, and how many are noted together
     const int tiles = (v1 - v0 + kTileVecs - 1) / kTileVecs;
@@ -478,10 +475,15 @@ logprobs_kernel(LogprobArgs a, int parts) {
     }
     if (n > 0) {
         if (warp == 0) {
-            // the n-th largest of 64 values, each the largest of four lanes' maxima, two to a lane here (equal ones in the order
-            // of all u, then all w)
-            const int4 p = *reinterpret_cast<const int4*>(lane_max + lane * 8), q = *reinterpret_cast<const int4*>(lane_max + lane * 8 + 4);
-            const int u = max(max(p.x, p.y), max(p.z, p.w)), w = max(max(q.x, q.y), max(q.z, q.w));
+            // the n-th largest of 64 values, each the largest of some lanes' maxima, two to a lane here (equal ones in the order of
+            // all u, then all w)
+            constexpr int kHalf = kThreads / 64;
+            int u = INT_MIN, w = INT_MIN;
+#pragma unroll
+            for (int q = 0; q < kHalf; q++) {
+                u = max(u, lane_max[lane * kHalf + q]);
+                w = max(w, lane_max[kThreads / 2 + lane * kHalf + q]);
+            }
             int place_u = 0, place_w = 0;
 #pragma unroll 4
             for (int o = 0; o < 32; o++) {
@@ -611,7 +613,7 @@ logprobs_kernel(LogprobArgs a, int parts) {
     }
 }
 
-template <typename T>
+template <typename T, int kWarps>
 cudaError_t launch(const LogprobArgs& a, int rows, int parts, cudaStream_t s) {
     static PerDeviceOnce once_large;
     cudaError_t e;
@@ -621,14 +623,14 @@ cudaError_t launch(const LogprobArgs& a, int rows, int parts, cudaStream_t s) {
         if (e != cudaSuccess) return e;
         const uint64_t bit = 1ull << (dev & 63);
         if (!(once_large.mask.load(std::memory_order_acquire) & bit)) {
-            e = cudaFuncSetAttribute(logprobs_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            e = cudaFuncSetAttribute(logprobs_kernel<T, kWarps>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
             if (e != cudaSuccess) return e;
             once_large.mask.fetch_or(bit, std::memory_order_release);
         }
     }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)rows * parts);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(kWarps * 32);
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -636,7 +638,7 @@ cudaError_t launch(const LogprobArgs& a, int rows, int parts, cudaStream_t s) {
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = parts > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, a, parts);
+    return cudaLaunchKernelEx(&cfg, logprobs_kernel<T, kWarps>, a, parts);
 }
 
 }  // namespace
@@ -645,13 +647,18 @@ int launch_logprobs(const void* logits, int dtype, int rows, int vocab, long lon
                     float* logprob, float* entropy, int32_t* rank, int32_t* top_ids, float* top_logprobs, int sm_count,
                     int32_t* bad_flag, int32_t* err, const Ctx& c) {
     LogprobArgs a{logits, stride, vocab, ids, ids_dtype, top_n, logprob, entropy, rank, top_ids, top_logprobs, bad_flag, err};
-    // CTAs per row: as many as keep every SM at four (clusters of more than eight do not pack that well: up to one per SM), each with
-    // two tiles of its own at least
-    const long long tiles = ((long long)vocab * (dtype == 0 ? 2 : 4) + kTileBytes - 1) / kTileBytes;
+    const int elem = dtype == 0 ? 2 : 4;
+    // Eight warps to a CTA; four where there are many rows that are short, for more of them at a time and less to join (4096 rows of
+    // 32003 bf16: 79 us against 89; 999 rows of 248320 bf16: 117 against 109)
+    const bool narrow = rows > 4 * sm_count && (long long)vocab * elem <= 8 * 8 * kWarpVecs * 16;
+    // CTAs per row: as many as keep every SM at 32 warps (clusters of more than eight CTAs do not pack that well: up to one per SM),
+    // each with two tiles of its own at least
+    const long long tiles = ((long long)vocab * elem + (narrow ? 4 : 8) * kWarpVecs * 16 - 1) / ((narrow ? 4 : 8) * kWarpVecs * 16);
     int parts = 1;
-    while (parts < kMaxCluster && (long long)rows * (parts + 1) <= (parts < 8 ? 4 * sm_count : sm_count) && tiles >= 2 * (parts + 1)) parts++;
+    while (parts < kMaxCluster && (long long)rows * (parts + 1) <= (parts < 8 ? (narrow ? 8 : 4) * sm_count : sm_count) && tiles >= 2 * (parts + 1)) parts++;
     c.begin(K_LOGPROBS);
-    const cudaError_t e = dtype == 0 ? launch<__nv_bfloat16>(a, rows, parts, c.s) : launch<float>(a, rows, parts, c.s);
+    const cudaError_t e = dtype == 0 ? (narrow ? launch<__nv_bfloat16, 4>(a, rows, parts, c.s) : launch<__nv_bfloat16, 8>(a, rows, parts, c.s))
+                                     : (narrow ? launch<float, 4>(a, rows, parts, c.s) : launch<float, 8>(a, rows, parts, c.s));
     c.end();
     return e == cudaSuccess ? 1 : -(int)e;
 }
