@@ -1263,12 +1263,14 @@ static int count_launches(ftm_handle* h, int n, const char* what) {
     return FTM_OK;
 }
 
+static constexpr int64_t kMaxExtent = 1 << 30;      // rows, columns: what 32-bit tile coordinates reach with room to spare
 static bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 static size_t act_bytes(int dtype) { return dtype == FTM_BF16 ? 2 : 4; }
 
 static int check_fp8_rows(const ftm_handle* h, const char* what, const void* x, int x_dtype, int64_t rows, int64_t k, int64_t stride) {
     if (x_dtype != FTM_BF16 && x_dtype != FTM_F32) return fail(h, FTM_ERR_BAD, "moe: %s: activations cannot be dtype %d", what, x_dtype);
-    if (rows <= 0 || k <= 0 || k % 16) return fail(h, FTM_ERR_BAD, "moe: %s: %lld rows of %lld (a nonzero multiple of 16)", what, (long long)rows, (long long)k);
+    if (rows <= 0 || rows > kMaxExtent || k <= 0 || k > kMaxExtent || k % 16)
+        return fail(h, FTM_ERR_BAD, "moe: %s: %lld rows of %lld (a nonzero multiple of 16; at most 2^30 of either)", what, (long long)rows, (long long)k);
     if (stride < k) return fail(h, FTM_ERR_BAD, "moe: %s: rows of %lld are %lld apart", what, (long long)k, (long long)stride);
     if (!aligned_to(x, act_bytes(x_dtype))) return fail(h, FTM_ERR_BAD, "moe: %s: activations not aligned to their type", what);
     return FTM_OK;
@@ -1276,7 +1278,7 @@ static int check_fp8_rows(const ftm_handle* h, const char* what, const void* x, 
 
 static int check_fp8_weight(const ftm_handle* h, const char* what, const void* w, const float* w_scale, int64_t n, const void* c, int c_dtype,
                             int64_t c_stride) {
-    if (n <= 0) return fail(h, FTM_ERR_BAD, "moe: %s: %lld weight rows", what, (long long)n);
+    if (n <= 0 || n > kMaxExtent) return fail(h, FTM_ERR_BAD, "moe: %s: %lld weight rows (at most 2^30)", what, (long long)n);
     if (c_dtype != FTM_BF16 && c_dtype != FTM_F32) return fail(h, FTM_ERR_BAD, "moe: %s: the output cannot be dtype %d", what, c_dtype);
     if (c_stride < n) return fail(h, FTM_ERR_BAD, "moe: %s: output rows of %lld are %lld apart", what, (long long)n, (long long)c_stride);
     if (!aligned_to(w, 16)) return fail(h, FTM_ERR_BAD, "moe: %s: the weight must be 16-byte aligned", what);
@@ -1309,7 +1311,8 @@ FTM_API int ftm_fp8_gemm(ftm_handle* h, const void* a_e4m3, const float* a_scale
     std::lock_guard<std::mutex> lk(h->mu);
     DeviceGuard dg(h->cfg.ordinal);
     if (!a_e4m3 || !a_scale || !w_e4m3 || !w_scale || !c) return fail(h, FTM_ERR_BAD, "moe: fp8 gemm: null buffer");
-    if (m <= 0 || k <= 0 || k % 16) return fail(h, FTM_ERR_BAD, "moe: fp8 gemm: %d rows of %d (a nonzero multiple of 16)", m, k);
+    if (m <= 0 || m > kMaxExtent || k <= 0 || k > kMaxExtent || k % 16)
+        return fail(h, FTM_ERR_BAD, "moe: fp8 gemm: %d rows of %d (a nonzero multiple of 16; at most 2^30 of either)", m, k);
     int rc = check_fp8_codes(h, "fp8 gemm", a_e4m3, a_scale);
     if (rc == FTM_OK) rc = check_fp8_weight(h, "fp8 gemm", w_e4m3, w_scale, n, c, c_dtype, c_stride);
     if (rc != FTM_OK) return rc;
@@ -1349,7 +1352,7 @@ FTM_API int ftm_logprobs(ftm_handle* h, const void* logits, int dtype, int32_t r
     DeviceGuard dg(h->cfg.ordinal);
     if (!logits) return fail(h, FTM_ERR_BAD, "moe: logprobs: null buffer");
     if (dtype != FTM_BF16 && dtype != FTM_F32) return fail(h, FTM_ERR_BAD, "moe: logprobs: logits cannot be dtype %d", dtype);
-    if (rows <= 0 || vocab <= 0 || vocab > (1 << 30)) return fail(h, FTM_ERR_BAD, "moe: logprobs: %d rows of %d logits", rows, vocab);
+    if (rows <= 0 || vocab <= 0 || vocab > (1 << 24)) return fail(h, FTM_ERR_BAD, "moe: logprobs: %d rows of %d logits (at most 2^24)", rows, vocab);
     if (row_stride < vocab) return fail(h, FTM_ERR_BAD, "moe: logprobs: rows of %d are %lld apart", vocab, (long long)row_stride);
     if (ids && ids_dtype != FTM_I32 && ids_dtype != FTM_I64) return fail(h, FTM_ERR_BAD, "moe: logprobs: token ids cannot be dtype %d", ids_dtype);
     if (!ids && (logprob_out || rank_out)) return fail(h, FTM_ERR_BAD, "moe: logprobs: a log probability or rank needs token ids");

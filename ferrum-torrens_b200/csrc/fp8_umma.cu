@@ -60,9 +60,6 @@ __device__ __forceinline__ void remote_store(uint32_t addr, const float* v, uint
                  "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])), "r"(bar)
                  : "memory");
 }
-__device__ __forceinline__ void remote_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_join() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 __device__ __forceinline__ bool cluster_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* err) {
@@ -150,7 +147,7 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     auto EMPTY = [&](int s) { return bar0 + 8u * (kMaxStages + s); };
     auto ACC_FULL = [&](int p) { return bar0 + 8u * (2 * kMaxStages + p); };
     auto ACC_EMPTY = [&](int p) { return bar0 + 8u * (2 * kMaxStages + kMaxAcc + p); };
-    const uint32_t SUM_FULL = bar0 + 8u * (2 * kMaxStages + 2 * kMaxAcc), SUM_FREE = SUM_FULL + 8;
+    const uint32_t SUM_FULL = bar0 + 8u * (2 * kMaxStages + 2 * kMaxAcc);
     uint32_t* const s_tmem = reinterpret_cast<uint32_t*>(bars + 2 * kMaxStages + 2 * kMaxAcc + 4);
     volatile int* const s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
 
@@ -168,7 +165,6 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
         if (lane < S::kAcc) mbar_init(ACC_FULL(lane), 2), mbar_init(ACC_EMPTY(lane), S::kEpi);
         if (lane == 0) {
             mbar_init(SUM_FULL, 1);
-            mbar_init(SUM_FREE, S::kEpi * split);
             *s_abort = 0;
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -312,11 +308,10 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     } else if (warp >= 4) {
         const int etid = threadIdx.x - 128, quarter = warp & 3, col0 = (warp - 4) / 4 * S::kCols;
         Ring p(S::kAcc);
-        uint32_t done = 0, got = 0;
         bool ok = true;
         const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + col0;
         const int row = quarter * 32 + lane;
-        for (int tile = first; tile < a.tiles && ok && warp < 4 + S::kEpi; tile += step, done++) {
+        for (int tile = first; tile < a.tiles && ok && warp < 4 + S::kEpi; tile += step) {
             const int n0 = tile / a.t_tiles * kRows, t0 = tile % a.t_tiles * NT;
             float acc[S::kCols];
 #pragma unroll
@@ -360,14 +355,12 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
                 }
                 continue;
             }
-            // the cluster's sums: the group of tokens 4 g .. 4 g + 3 belongs to the CTA g / share.  A lane is a weight row, so its four
+            // the cluster's sums (a cluster has one tile): the group of tokens 4 g .. 4 g + 3 belongs to the CTA g / share.  A lane is a weight row, so its four
             // sums of a group are one store of 16 bytes, beside its neighbours'.
             const int share = S::share(split), groups = (min(NT, a.M - t0) + 3) / 4, mine = min(share, groups - rank * share);
-            const bool last = tile + step >= a.tiles;
             if (etid == 0 && mine > 0) mbar_expect_tx(SUM_FULL, split * mine * kRows * 16);
-            if (!joined) cluster_join(), joined = true;
-            if (done > 0) ok = __all_sync(0xffffffffu, cluster_wait(SUM_FREE, (done - 1) & 1, s_abort, a.err));
-            if (!ok) break;
+            cluster_join();
+            joined = true;
             const uint32_t my_sums = smem_u32(sums + (rank * share * kRows + row) * 4);
             uint32_t to_sums = 0, to_bar = 0;
             int to = col0 / 4 / share, in_share = col0 / 4 - to * share;
@@ -379,9 +372,10 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
                 if (++in_share == share) in_share = 0, to++;
             }
             __syncwarp();
-            if (last) cluster_arrive(), left = true;      // nothing of this warp's goes to another CTA from here on
+            cluster_arrive();      // nothing of this warp's goes to another CTA from here on
+            left = true;
             if (mine > 0) {
-                ok = __all_sync(0xffffffffu, cluster_wait(SUM_FULL, got++ & 1, s_abort, a.err));
+                ok = __all_sync(0xffffffffu, cluster_wait(SUM_FULL, 0, s_abort, a.err));
                 if (!ok) break;
                 for (int q = etid; q < mine * kRows; q += 32 * S::kEpi) {
                     const int g = q / kRows, n = q % kRows, t = t0 + (rank * share + g) * 4;
@@ -400,8 +394,6 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
                     }
                 }
             }
-            __syncwarp();
-            if (!last && lane < split) remote_arrive(map_shared_to(SUM_FREE, lane));
         }
     }
     if (!joined) cluster_join();
@@ -412,6 +404,12 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     if (split > 1) cluster_join();
 }
 
+template <int NT, bool FUSED>
+cudaError_t prepare() {
+    static PerDeviceOnce once;
+    return allow_dyn_smem(once, fp8_umma_kernel<NT, FUSED>, 227 * 1024);
+}
+
 // Clusters of q CTAs that the device holds at a time (SMs are grouped, so eights and sevens leave some of them empty)
 template <int NT, bool FUSED>
 int clusters_at_once(int q) {
@@ -420,6 +418,7 @@ int clusters_at_once(int q) {
     if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return 0;
     int n = known[dev][q].load(std::memory_order_relaxed);
     if (n) return n;
+    if (prepare<NT, FUSED>() != cudaSuccess) return 0;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(q);
     cfg.blockDim = dim3(Shape<NT, FUSED>::kThreads);
@@ -462,8 +461,7 @@ int launch(const uint8_t* codes, const uint8_t* w, Fp8Args a, int sm_count, cuda
     a.blocks = (a.K + kFp8Block - 1) / kFp8Block;
     a.t_tiles = (a.M + NT - 1) / NT;
     a.tiles = a.t_tiles * ((a.N + kRows - 1) / kRows);
-    static PerDeviceOnce once;
-    cudaError_t e = allow_dyn_smem(once, fp8_umma_kernel<NT, FUSED>, 227 * 1024);
+    cudaError_t e = prepare<NT, FUSED>();
     if (e != cudaSuccess) return -(int)e;
     const Plan plan = plan_for<NT, FUSED>(a.M, a.N, a.blocks, sm_count);
     const int split = plan.split;
@@ -478,7 +476,7 @@ int launch(const uint8_t* codes, const uint8_t* w, Fp8Args a, int sm_count, cuda
     if (!fp8_codes_map(&map_w, w, a.N, a.K, kRows) || (!FUSED && !fp8_codes_map(&map_a, codes, a.M, a.K, NT))) return -(int)cudaErrorInvalidValue;
     if (FUSED) map_a = map_w;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(split * max(1, min(a.tiles, S::kPerSm * sm_count / split)));
+    cfg.gridDim = dim3(split > 1 ? split * a.tiles : min(a.tiles, S::kPerSm * sm_count));
     cfg.blockDim = dim3(S::kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;

@@ -35,7 +35,7 @@ constexpr float kInf = __builtin_huge_valf();
 constexpr float kFar = -1e20f;       // differences below this have exponential 0; clamped there, sums of them stay finite
 constexpr int kCandidates = 512;
 constexpr int kNotes = 64;           // noted maxima of a warp; longer parts note several tiles together
-constexpr uint32_t kSpin = 1u << 20; // looks at a barrier before a wait is given up
+constexpr uint32_t kSpin = 1u << 24; // looks at a barrier before a wait is given up (a part full of ties takes some ms longer than the others)
 
 __device__ __forceinline__ float ex2(float v) {
     float r;

@@ -181,6 +181,7 @@ class B200MoE:
         self.experts, self.layers, self.top_k = experts, layers, top_k
         self.shared_inter, self.max_tokens = shared_inter, max_tokens
         self.device = device
+        self._own_stream = 0 if stream is None else stream if isinstance(stream, int) else stream.cuda_stream
         cfg = L.Config(device, shapes.hidden, shapes.inter, top_k, experts, layers, slots, shared_inter, max_tokens,
                        ep_rank, ep_size)
         sp = _stream_ptr(stream) if stream is not None else C.c_void_p(0)
@@ -631,6 +632,17 @@ class B200MoE:
             return _current_stream()(self.device)
         return stream if isinstance(stream, int) else stream.cuda_stream
 
+    def _lend(self, tensors, on: int):
+        """Tensors made here for a call on stream `on`: where that is not the stream they were made on, their memory is not handed
+        out again before the call is done."""
+        on = on or self._own_stream
+        if on != _current_stream()(self.device):
+            torch = _torch()
+            there = torch.cuda.ExternalStream(on, device=self.device) if on else torch.cuda.default_stream(self.device)
+            for t in tensors:
+                if t is not None:
+                    t.record_stream(there)
+
     def _rows(self, t, what: str, codes: dict, shape=None) -> int:
         """Address of a matrix on this adapter's device whose last dimension is contiguous; its rows may be apart."""
         if (t.dtype in codes and t.get_device() == self.device and t.dim() == 2 and (shape is None or t.shape == shape)
@@ -659,10 +671,11 @@ class B200MoE:
         ty = _types()
         px = self._rows(x, "x", ty.act)
         m, k = x.shape
-        q, scale = out = self._fp8_pair(x, m, k) if out is None else out
+        on = self._on(stream)
+        q, scale = out = self._fp8_pair(x, m, k, on) if out is None else out
         pq = self._flat(q, "the codes", ty.e4m3, (m, k))
         ps = self._flat(scale, "the scales", ty.f32, (-(-k // 128), m))
-        rc = self._lib.ftm_fp8_quantize(self._h, px, ty.act[x.dtype], m, k, x.stride(0) if m > 1 else k, pq, ps, self._on(stream))
+        rc = self._lib.ftm_fp8_quantize(self._h, px, ty.act[x.dtype], m, k, x.stride(0) if m > 1 else k, pq, ps, on)
         if rc:
             self._check(rc)
         return out
@@ -686,23 +699,26 @@ class B200MoE:
         ty = _types()
         px = self._rows(x, "x", ty.act)
         m, n, k, blocks, pw, pws, pc = self._fp8_operands(ty, x, w, w_scale, out)
+        on = self._on(stream)
         if scratch is None and (m > 16 or k > 8192):
-            scratch = self._fp8_pair(x, m, k)
+            scratch = self._fp8_pair(x, m, k, on)
         pq = ps = None
         if scratch is not None:
             pq = self._flat(scratch[0], "the codes", ty.e4m3, (m, k))
             ps = self._flat(scratch[1], "the scales", ty.f32, (blocks, m))
         rc = self._lib.ftm_fp8_linear(self._h, px, ty.act[x.dtype], x.stride(0) if m > 1 else k, pw, pws, m, n, k, pq, ps, pc, ty.act[out.dtype],
-                                      out.stride(0) if m > 1 else n, self._on(stream))
+                                      out.stride(0) if m > 1 else n, on)
         if rc:
             self._check(rc)
         return out
 
-    def _fp8_pair(self, x, m: int, k: int):
-        """Room for the codes and scales of m rows of k."""
+    def _fp8_pair(self, x, m: int, k: int, on: int):
+        """Room for the codes and scales of m rows of k, for a call on stream `on`."""
         torch = _torch()
-        return (torch.empty((m, k), dtype=torch.float8_e4m3fn, device=x.device),
+        made = (torch.empty((m, k), dtype=torch.float8_e4m3fn, device=x.device),
                 torch.empty((-(-k // 128), m), dtype=torch.float32, device=x.device))
+        self._lend(made, on)
+        return made
 
     def _fp8_operands(self, ty, a, w, w_scale, out):
         """Sizes and addresses that fp8_gemm and fp8_linear have in common."""
@@ -724,21 +740,23 @@ class B200MoE:
         rows, vocab = logits.shape
         if not 0 <= top_n <= 32:
             raise bad(f"logprobs: {top_n} alternatives (at most 32)")
+        flat, shape = self._flat, (rows,)
+        pi = None if ids is None else flat(ids, "the token ids", ty.ids, shape)
+        on = self._on(stream)
         if out is None:
             torch = _torch()
             new = lambda dtype, *shape: torch.empty(shape, dtype=dtype, device=logits.device)
             out = (new(torch.float32, rows) if ids is not None else None, new(torch.float32, rows),
                    new(torch.int32, rows) if ids is not None else None, new(torch.int32, rows, top_n), new(torch.float32, rows, top_n))
+            self._lend(out, on)
         lp, entropy, rank, top_ids, top_lp = out
-        flat, shape = self._flat, (rows,)
-        pi = None if ids is None else flat(ids, "the token ids", ty.ids, shape)
         p1 = None if lp is None else flat(lp, "the log probabilities", ty.f32, shape)
         p2 = None if entropy is None else flat(entropy, "the entropies", ty.f32, shape)
         p3 = None if rank is None else flat(rank, "the ranks", ty.i32, shape)
         p4 = None if top_ids is None else flat(top_ids, "the alternatives", ty.i32, (rows, top_n))
         p5 = None if top_lp is None else flat(top_lp, "the alternatives' log probabilities", ty.f32, (rows, top_n))
         rc = self._lib.ftm_logprobs(self._h, px, ty.act[logits.dtype], rows, vocab, logits.stride(0) if rows > 1 else vocab, pi,
-                                    L.I32 if ids is None else ty.ids[ids.dtype], top_n, p1, p2, p3, p4, p5, self._on(stream))
+                                    L.I32 if ids is None else ty.ids[ids.dtype], top_n, p1, p2, p3, p4, p5, on)
         if rc:
             self._check(rc)
         return out

@@ -262,14 +262,15 @@ FTM_API int ftm_dense_gemv(ftm_handle* h, const void* a, int a_dtype, const void
  *   a0 = max(largest magnitude of the block, 448 * 2^-126),  scale = a0 / 448,  q = e4m3(x * (448 / a0))
  * in f32, rounded to the nearest code, ties to even; a NaN stays one and does not count as a magnitude, a block with an
  * infinity has scale infinity and codes 0 and NaN.  x [rows, k] bf16 or f32 dev, its rows x_stride elements apart;
- * q [rows, k] e4m3 dev, 16-byte aligned; scale [ceil(k / 128), rows] f32 dev.  k a multiple of 16.  Asynchronous. */
+ * q [rows, k] e4m3 dev, 16-byte aligned; scale [ceil(k / 128), rows] f32 dev.  k a multiple of 16; rows and k at most 2^30.
+ * As in the calls below, outputs overlap no input.  Asynchronous. */
 FTM_API int ftm_fp8_quantize(ftm_handle* h, const void* x, int x_dtype, int32_t rows, int32_t k, int64_t x_stride, void* q_e4m3,
                              float* scale, void* stream);
 /* c[t, n] = sum over blocks b of 128 k of  a_scale[b, t] * w_scale[n / 128, b] * sum_{k in b} a[t, k] * w[n, k],
  * every sum in f32, c rounded once.  a [m, k] and a_scale as ftm_fp8_quantize writes them; w [n, k] e4m3 dev and w_scale
  * [ceil(n / 128), ceil(k / 128)] f32 dev, the layout of checkpoints in 8 bits; a and w 16-byte aligned.  c [m, n] bf16 or
- * f32 dev, its rows c_stride elements apart (what lies between n and c_stride is not written).  k a multiple of 16, any
- * m and n.  The same inputs give the same bits.  Asynchronous. */
+ * f32 dev, its rows c_stride elements apart (what lies between n and c_stride is not written).  k a multiple of 16; any m
+ * and n; each at most 2^30.  The same inputs give the same bits.  Asynchronous. */
 FTM_API int ftm_fp8_gemm(ftm_handle* h, const void* a_e4m3, const float* a_scale, const void* w_e4m3, const float* w_scale, int32_t m,
                          int32_t n, int32_t k, void* c, int c_dtype, int64_t c_stride, void* stream);
 /* ftm_fp8_gemm of ftm_fp8_quantize(x) in one call; for up to 16 rows of up to 8192 elements in one kernel, which needs no scratch
@@ -280,7 +281,7 @@ FTM_API int ftm_fp8_linear(ftm_handle* h, const void* x, int x_dtype, int64_t x_
                            int64_t c_stride, void* stream);
 
 /* ---- what a server reads off its logits (no counterpart in the reference) ------------------------------------ */
-/* logits [rows, vocab] bf16 or f32 dev, rows row_stride elements apart (as ftm_dense_gemv or ftm_fp8_linear leave them);
+/* logits [rows, vocab] bf16 or f32 dev (vocab at most 2^24), rows row_stride elements apart (as ftm_dense_gemv or ftm_fp8_linear leave them);
  * ids [rows] i32 or i64 dev, one token per row.  Per row, with all sums in f32:
  *   logprob_out   log softmax(logits)[id]
  *   entropy_out   -sum p log p  (an element of -inf adds nothing)

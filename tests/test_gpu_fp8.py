@@ -96,6 +96,16 @@ def test_quantize_is_the_formula_bit_for_bit(moe, m, k, pad, offset, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("m,k,pad", [(5000, 2064, 0), (1203, 8192, 8), (4999, 144, 3)])
+def test_quantize_walks_over_large_inputs(moe, m, k, pad, dtype):
+    x = activations(m + k, m, k, DT[dtype], pad)
+    q, s = moe.fp8_quantize(x)
+    want_q, want_s = quantised(x)
+    assert np.array_equal(s.cpu().numpy(), want_s)
+    assert np.array_equal(q.float().cpu().numpy(), want_q.astype(np.float32))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_quantize_special_values(moe, dtype):
     big, tiny = torch.finfo(DT[dtype]).max, torch.finfo(DT[dtype]).smallest_normal
     rows = torch.zeros((8, 272))
@@ -174,6 +184,43 @@ def test_linear_is_the_product_of_the_quantised_rows(moe, m, n, k, pad, offset, 
     moe.fp8_linear(rows, w, ws, again, scratch=scratch)
     assert torch.equal(again, c)
     moe.sync_status()
+
+
+@pytest.mark.parametrize("sms", [1, 2, 7, 40])
+@pytest.mark.parametrize("m", [3, 30, 50, 120, 300, 700])
+def test_few_sms(moe, m, sms):
+    """A budget of SMs: few CTAs walk over many tiles, and the blocks are split less or not at all."""
+    n, k = 1500, 1040
+    x = activations(m, m, k, torch.bfloat16).contiguous()
+    w, ws = weight(m + 1, n, k)
+    q, s = quantised(x)
+    moe.set_sm_budget(sms)
+    try:
+        for out in (torch.float32, torch.bfloat16):
+            c = torch.full((m, n), 77.0, dtype=out, device=DEV)
+            moe.fp8_linear(x, w, ws, c)
+            check_product(c, q, s, w, ws)
+            c2 = torch.empty_like(c)
+            moe.fp8_gemm(*moe.fp8_quantize(x), w, ws, c2)
+            check_product(c2, q, s, w, ws)
+        moe.sync_status()
+    finally:
+        moe.set_sm_budget(0)
+
+
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+@pytest.mark.parametrize("n,ld,offset", [(512, 512, 0), (512, 520, 0), (512, 516, 0), (515, 517, 1), (514, 522, 2), (300, 301, 0), (600, 604, 4)])
+def test_output_rows_of_any_alignment(moe, n, ld, offset, out):
+    m, k = 400, 256
+    q, s = moe.fp8_quantize(activations(n, m, k, torch.bfloat16))
+    w, ws = weight(ld, n, k)
+    buf = torch.full((m * ld + offset + 9,), 77.0, dtype=DT[out], device=DEV)
+    c = buf[offset:].as_strided((m, n), (ld, 1), storage_offset=offset)
+    moe.fp8_gemm(q, s, w, ws, c)
+    check_product(c, q.double().cpu().numpy(), s.cpu().numpy(), w, ws)
+    kept = torch.ones_like(buf, dtype=torch.bool)
+    kept.as_strided((m, n), (ld, 1), storage_offset=offset).fill_(False)
+    assert (buf[kept] == 77.0).all()
 
 
 @pytest.mark.parametrize("m", [1, 9, 40, 130, 600])
@@ -267,6 +314,38 @@ def test_graphs_streams_and_chained_calls(moe):
     moe.sync_status()
 
 
+def test_scratch_made_for_another_stream_is_not_handed_out_early(moe):
+    """Without scratch of its own a call on a side stream must not see it reused by what the current stream allocates meanwhile."""
+    m, n, k = 64, 256, 2048
+    x, (w, ws) = activations(1, m, k, torch.bfloat16), weight(2, n, k)
+    want = torch.empty((m, n), device=DEV)
+    moe.fp8_linear(x, w, ws, want)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for given in (side, side.cuda_stream):
+        c = torch.zeros((m, n), device=DEV)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+        moe.fp8_linear(x, w, ws, c, stream=given)
+        q, s = moe.fp8_quantize(x, stream=given)
+        del q, s
+        junk = [torch.full((m, k), 0x7f, dtype=torch.uint8, device=DEV) for _ in range(8)] + [torch.full((k // 128, m), 9e9, device=DEV) for _ in range(8)]
+        torch.cuda.synchronize()
+        assert torch.equal(c, want) and len(junk) == 16
+    # an adapter with a stream of its own takes the default stream's place
+    own = pkg.B200MoE(0, pkg.ExpertShapes(64, 16), 1, experts=1, layers=1, top_k=1, shared_inter=16, max_tokens=1, stream=side)
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+    c = torch.zeros((m, n), device=DEV)
+    side.wait_stream(torch.cuda.current_stream())
+    own.fp8_linear(x, w, ws, c)
+    junk = [torch.full((m, k), 0x7f, dtype=torch.uint8, device=DEV) for _ in range(8)]
+    torch.cuda.synchronize()
+    assert torch.equal(c, want) and junk
+    own.close()
+
+
 def test_refusals(moe):
     x = torch.zeros((4, 256), dtype=torch.bfloat16, device=DEV)
     w, ws = weight(0, 130, 256)
@@ -297,5 +376,16 @@ def test_refusals(moe):
     assert quant() == L.OK
     for kw in (dict(px=null), dict(pq=null), dict(ps=null), dict(dt=L.I64), dict(m=0), dict(k=8), dict(ld=255), dict(px=p(x, 1)), dict(pq=p(q, 4)), dict(ps=p(s, 1))):
         assert quant(**kw) == L.ERR_BAD, kw
+    linear = lambda px=p(x), dt=L.BF16, ld=256, pw=p(w), sw=p(ws), m=4, n=130, k=256, pq=null, ps=null, pc=p(c), ct=L.F32, cl=130: lib.ftm_fp8_linear(
+        h, px, dt, ld, pw, sw, m, n, k, pq, ps, pc, ct, cl, st)
+    assert linear() == L.OK
+    many = torch.zeros((17, 256), dtype=torch.bfloat16, device=DEV)
+    cm, (qm, sm) = torch.empty((17, 130), device=DEV), moe.fp8_quantize(many)
+    big = dict(px=p(many), m=17, pc=p(cm))
+    assert linear(**big, pq=p(qm), ps=p(sm)) == L.OK
+    for kw in (dict(px=null), dict(pw=null), dict(sw=null), dict(pc=null), dict(m=0), dict(n=0), dict(k=0), dict(k=8), dict(dt=L.I32), dict(ct=L.I64), dict(ld=255),
+               dict(cl=129), dict(pw=p(w, 8)), dict(px=p(x, 1)), dict(m=2 ** 30 + 1), dict(n=2 ** 30 + 1, cl=2 ** 31), dict(k=2 ** 30 + 16, ld=2 ** 31),
+               big, dict(**big, pq=p(qm)), dict(**big, ps=p(sm)), dict(**big, pq=p(qm, 8), ps=p(sm)), dict(**big, pq=p(qm), ps=p(sm, 2))):
+        assert linear(**kw) == L.ERR_BAD, kw
     assert lib.ftm_fp8_gemm(null, null, null, null, null, 1, 1, 16, null, 0, 1, null) == L.ERR_BAD
     torch.cuda.synchronize()

@@ -96,7 +96,7 @@ def check(moe, x, ids, n, ids_dtype=torch.int64):
 @pytest.mark.parametrize("rows,vocab,n,pad,offset", [
     (1, 1, 1, 0, 0), (2, 2, 5, 0, 0), (3, 7, 7, 2, 1), (3, 31, 32, 0, 0), (1, 33, 20, 0, 0), (5, 1000, 0, 0, 0), (5, 1000, 1, 3, 2), (2, 4097, 20, 0, 0),
     (1, 40000, 32, 0, 0), (300, 513, 5, 0, 0), (3, 40001, 20, 7, 3), (700, 1500, 3, 0, 0), (1, 248320, 20, 0, 0), (2, 100003, 8, 0, 0), (9, 65536, 9, 64, 0),
-    (40, 33000, 17, 1, 0)])
+    (40, 33000, 17, 1, 0), (650, 40001, 12, 0, 0), (800, 9000, 32, 5, 1), (13, 248320, 20, 0, 0), (150, 70000, 2, 0, 0)])
 def test_random_rows(moe, rows, vocab, n, pad, offset, dtype):
     x = logits_of(rows + vocab, rows, vocab, DT[dtype], pad, offset)
     gen = torch.Generator(device=DEV).manual_seed(vocab)
