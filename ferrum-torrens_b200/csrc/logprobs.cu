@@ -247,45 +247,23 @@ __device__ __forceinline__ int larger_than(const uint64_t* keys, int count, uint
     return place;
 }
 
-// The best n <= 32 of up to 16 sorted lists (0 ends one), by one warp, which gets them in its lanes.  The first two entries of
-// each list, or as many as make n, give a bound that n of them reach; what reaches it is moved together and placed by
-// counting.  room: lists * 32 keys, aligned to 16 bytes; best: 32 keys.
-__device__ __forceinline__ uint64_t merge_lists(const uint64_t (*list)[32], int lists, int n, int lane, uint64_t* room, uint64_t* best) {
-    const int deep = max(2, (n + lists - 1) / lists);
-    uint64_t bound = 0;
-    if (lists * deep <= 32) {
-        const uint64_t e = lane < lists * deep ? list[lane / deep][lane % deep] : 0;
-        int place = 0;
-#pragma unroll 8
-        for (int o = 0; o < 32; o++) {
-            const uint64_t other = __shfl_sync(0xffffffffu, e, o);
-            place += (int)(other > e) | (int)((other == e) & (o < lane));
+// The best n <= 32 of up to 32 sorted lists (0 ends one), by one warp, which gets them in its lanes: n times the best of the heads.
+// (Code that runs once per row is kept short: what it takes to fetch its instructions is most of its time.)
+__device__ __forceinline__ uint64_t merge_lists(const uint64_t (*list)[32], int lists, int n, int lane) {
+    int at = 0;
+    uint64_t head = lane < lists ? list[lane][0] : 0, mine = 0;
+#pragma unroll 1
+    for (int q = 0; q < n; q++) {
+        const uint32_t high = __reduce_max_sync(0xffffffffu, (uint32_t)(head >> 32));
+        const uint32_t low = __reduce_max_sync(0xffffffffu, (uint32_t)(head >> 32) == high ? (uint32_t)head : 0u);
+        const uint64_t best = (uint64_t)high << 32 | low;
+        if (lane == q) mine = best;
+        if (head == best) {
+            at++;
+            head = at < n && lane < lists ? list[lane][at] : 0;
         }
-        bound = __shfl_sync(0xffffffffu, e, __ffs(__ballot_sync(0xffffffffu, place == n - 1)) - 1);
     }
-    int mine = 0;
-    if (lane < lists)
-        while (mine < n && list[lane][mine] >= bound && list[lane][mine] != 0) mine++;
-    int at = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int below = __shfl_up_sync(0xffffffffu, at, o);
-        if (lane >= o) at += below;
-    }
-    const int count = __shfl_sync(0xffffffffu, at, 31);
-    at -= mine;
-    for (int q = 0; q < mine; q++) room[at + q] = list[lane][q];
-    __syncwarp();
-    // (an entry's place is found by its lane; the n-th and those before it end up in the lanes)
-    best[lane] = 0;
-    __syncwarp();
-    for (int q = lane; q < count; q += 32) {
-        const uint64_t k = room[q];
-        const int place = larger_than(room, count, k);
-        if (place < n) best[place] = k;
-    }
-    __syncwarp();
-    return best[lane];
+    return mine;
 }
 
 // ---- sending results to the first CTA of the cluster -------------------------------------------
@@ -475,8 +453,7 @@ logprobs_kernel(LogprobArgs a, int parts) {
     }
     if (n > 0) {
         if (warp == 0) {
-            // the n-th largest of 64 values, each the largest of some lanes' maxima, two to a lane here (equal ones in the order of
-            // all u, then all w)
+            // the n-th largest of 64 values, each the largest of some lanes' maxima, two to a lane here
             constexpr int kHalf = kThreads / 64;
             int u = INT_MIN, w = INT_MIN;
 #pragma unroll
@@ -484,15 +461,16 @@ logprobs_kernel(LogprobArgs a, int parts) {
                 u = max(u, lane_max[lane * kHalf + q]);
                 w = max(w, lane_max[kThreads / 2 + lane * kHalf + q]);
             }
-            int place_u = 0, place_w = 0;
-#pragma unroll 4
-            for (int o = 0; o < 32; o++) {
-                const int ou = __shfl_sync(0xffffffffu, u, o), ow = __shfl_sync(0xffffffffu, w, o);
-                place_u += ((ou > u) | ((ou == u) & (o < lane))) + (ow > u);
-                place_w += (ou >= w) + ((ow > w) | ((ow == w) & (o < lane)));
+            int best = INT_MIN;
+#pragma unroll 1
+            for (int q = 0; q < n; q++) {
+                best = __reduce_max_sync(0xffffffffu, max(u, w));
+                if (lane == __ffs(__ballot_sync(0xffffffffu, max(u, w) == best)) - 1) {
+                    if (u == best) u = INT_MIN;
+                    else w = INT_MIN;
+                }
             }
-            if (place_u == n - 1) s_bound = u;
-            if (place_w == n - 1) s_bound = w;
+            if (lane == 0) s_bound = best;
         }
         __syncthreads();
         const float bound = from_ordered(s_bound);
@@ -568,7 +546,7 @@ logprobs_kernel(LogprobArgs a, int parts) {
         }
     }
     uint64_t mine = best[lane];
-    if (parts > 1 && n > 0) mine = merge_lists(lists, parts, n, lane, found, best);
+    if (parts > 1 && n > 0) mine = merge_lists(lists, parts, n, lane);
     Stats all;
     int rank = 0;
     if (lane < parts) {
