@@ -97,6 +97,13 @@ __device__ __forceinline__ void fp8_encode(const Fp8Eight<T> (&f)[U], uint2 (&co
     }
 }
 
+// A CTA in which a wait gave up stays for about a millisecond: its copies and products still in flight take microseconds.
+__device__ __forceinline__ void fp8_settle(const volatile int* gave_up) {
+    if (!*gave_up) return;
+    const long long from = clock64();
+    while (clock64() - from < 2000000) {}
+}
+
 inline bool fp8_rows_aligned(const void* x, int x_dtype, long long stride) {
     return reinterpret_cast<uintptr_t>(x) % 16 == 0 && stride * (x_dtype == 0 ? 2 : 4) % 16 == 0;
 }

@@ -158,96 +158,96 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
-    if (warp == 0) {
-        int st = 0;
-        uint32_t round = 0;
-        bool ok = true;
-        for (int tile = first; tile < a.tiles && ok; tile += step) {
-            const int t0 = tile % a.m_tiles * kM + rank * 128, n0 = tile / a.m_tiles * kN + rank * 128;
-            for (int kb = 0; kb < a.blocks; kb++) {
-                ok = mbar_wait_warp(EMPTY(st), round ^ 1, s_abort, a.err);
-                if (!ok) break;
-                if (elect_one()) {
-                    const uint32_t dst = smem_u32(ring + st * kStage), bar = in_first_cta(FULL(st));
-                    // the bytes of both CTAs; what a box reads past the matrix is zero and counts all the same
-                    if (rank == 0) mbar_expect_tx(FULL(st), 2 * kStage);
-                    tma_load_pair(dst, &tmap_a, kb * kFp8Block, t0, bar);
-                    tma_load_pair(dst + kHalfBytes, &tmap_w, kb * kFp8Block, n0, bar);
-                }
-                __syncwarp();
-                if (++st == kStages) st = 0, round ^= 1;
-            }
-        }
-    } else if (warp == 1 || warp == 3) {
-        // two issuers: the wait and the issue of one block take one warp longer than the products themselves
-        if (rank == 0) {
-            int st = 0, p = 0;
-            uint32_t round = 0, p_round = 0;
-            bool ok = true, my_turn = warp == 1;
+        if (warp == 0) {
+            int st = 0;
+            uint32_t round = 0;
+            bool ok = true;
             for (int tile = first; tile < a.tiles && ok; tile += step) {
-                for (int kb = 0; kb < a.blocks; kb++, my_turn = !my_turn) {
-                    if (my_turn) {
-                        ok = mbar_wait_warp(FULL(st), round, s_abort, a.err) && mbar_wait_warp(ACC_EMPTY(p), p_round ^ 1, s_abort, a.err);
-                        if (!ok) break;
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        const uint32_t base = smem_u32(ring + st * kStage);
-                        const uint64_t adesc = umma_desc(base), wdesc = umma_desc(base + kHalfBytes);
-                        if (elect_one()) {
-#pragma unroll
-                            for (int kk = 0; kk < 4; kk++) umma_f8_pair(tmem_base + p * kN, adesc + kk * 2, wdesc + kk * 2, kk > 0);
-                            commit_pair(ACC_FULL(p));
-                            commit_pair(EMPTY(st));
-                        }
-                        __syncwarp();
+                const int t0 = tile % a.m_tiles * kM + rank * 128, n0 = tile / a.m_tiles * kN + rank * 128;
+                for (int kb = 0; kb < a.blocks; kb++) {
+                    ok = mbar_wait_warp(EMPTY(st), round ^ 1, s_abort, a.err);
+                    if (!ok) break;
+                    if (elect_one()) {
+                        const uint32_t dst = smem_u32(ring + st * kStage), bar = in_first_cta(FULL(st));
+                        // the bytes of both CTAs; what a box reads past the matrix is zero and counts all the same
+                        if (rank == 0) mbar_expect_tx(FULL(st), 2 * kStage);
+                        tma_load_pair(dst, &tmap_a, kb * kFp8Block, t0, bar);
+                        tma_load_pair(dst + kHalfBytes, &tmap_w, kb * kFp8Block, n0, bar);
                     }
+                    __syncwarp();
                     if (++st == kStages) st = 0, round ^= 1;
-                    if (++p == 2) p = 0, p_round ^= 1;
+                }
+            }
+        } else if (warp == 1 || warp == 3) {
+            // two issuers: the wait and the issue of one block take one warp longer than the products themselves
+            if (rank == 0) {
+                int st = 0, p = 0;
+                uint32_t round = 0, p_round = 0;
+                bool ok = true, my_turn = warp == 1;
+                for (int tile = first; tile < a.tiles && ok; tile += step) {
+                    for (int kb = 0; kb < a.blocks; kb++, my_turn = !my_turn) {
+                        if (my_turn) {
+                            ok = mbar_wait_warp(FULL(st), round, s_abort, a.err) && mbar_wait_warp(ACC_EMPTY(p), p_round ^ 1, s_abort, a.err);
+                            if (!ok) break;
+                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                            const uint32_t base = smem_u32(ring + st * kStage);
+                            const uint64_t adesc = umma_desc(base), wdesc = umma_desc(base + kHalfBytes);
+                            if (elect_one()) {
+#pragma unroll
+                                for (int kk = 0; kk < 4; kk++) umma_f8_pair(tmem_base + p * kN, adesc + kk * 2, wdesc + kk * 2, kk > 0);
+                                commit_pair(ACC_FULL(p));
+                                commit_pair(EMPTY(st));
+                            }
+                            __syncwarp();
+                        }
+                        if (++st == kStages) st = 0, round ^= 1;
+                        if (++p == 2) p = 0, p_round ^= 1;
+                    }
+                }
+            }
+        } else {
+            // two blocks' scales are asked for at a time, and the next two before these are handed out
+            int p = 0;
+            uint32_t p_round = 0;
+            bool ok = true;
+            float now[2][4], next[2][4], now_w[2][2], next_w[2][2];
+            for (int tile = first; tile < a.tiles && ok; tile += step) {
+                const int t0 = tile % a.m_tiles * kM + rank * 128 + lane, nb = tile / a.m_tiles * 2;
+                const bool second = (nb + 1) * kFp8Block < a.N;
+                const float* const sw = a.w_scale + (size_t)nb * a.blocks;
+                auto ask = [&](int kb0, float (&v)[2][4], float (&w)[2][2]) {
+#pragma unroll
+                    for (int q = 0; q < 2; q++) {
+                        const int kb = kb0 + q;
+                        w[q][0] = kb < a.blocks ? __ldg(sw + kb) : 0.f;
+                        w[q][1] = kb < a.blocks && second ? __ldg(sw + a.blocks + kb) : 0.f;
+#pragma unroll
+                        for (int j = 0; j < 4; j++) v[q][j] = kb < a.blocks && t0 + 32 * j < a.M ? __ldcg(a.a_scale + (size_t)kb * a.M + t0 + 32 * j) : 0.f;
+                    }
+                };
+                ask(0, now, now_w);
+                for (int kb0 = 0; kb0 < a.blocks && ok; kb0 += 2) {
+                    ask(kb0 + 2, next, next_w);
+#pragma unroll
+                    for (int q = 0; q < 2; q++) {
+                        if (kb0 + q >= a.blocks || !ok) continue;
+                        ok = mbar_wait_warp(SLOT_EMPTY(p), p_round ^ 1, s_abort, a.err);
+                        if (!ok) continue;
+#pragma unroll
+                        for (int j = 0; j < 4; j++) slots[p * 130 + lane + 32 * j] = now[q][j];
+                        if (lane < 2) slots[p * 130 + 128 + lane] = lane ? now_w[q][1] : now_w[q][0];
+                        mbar_arrive_warp(ACC_FULL(p));
+                        if (++p == 2) p = 0, p_round ^= 1;
+                    }
+#pragma unroll
+                    for (int q = 0; q < 2; q++) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) now[q][j] = next[q][j];
+                        now_w[q][0] = next_w[q][0], now_w[q][1] = next_w[q][1];
+                    }
                 }
             }
         }
-    } else {
-        // four blocks' scales are asked for at a time, and the next four before these are handed out
-        int p = 0;
-        uint32_t p_round = 0;
-        bool ok = true;
-        float now[4][4], next[4][4], now_w[4][2], next_w[4][2];
-        for (int tile = first; tile < a.tiles && ok; tile += step) {
-            const int t0 = tile % a.m_tiles * kM + rank * 128 + lane, nb = tile / a.m_tiles * 2;
-            const bool second = (nb + 1) * kFp8Block < a.N;
-            const float* const sw = a.w_scale + (size_t)nb * a.blocks;
-            auto ask = [&](int kb0, float (&v)[4][4], float (&w)[4][2]) {
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const int kb = kb0 + q;
-                    w[q][0] = kb < a.blocks ? __ldg(sw + kb) : 0.f;
-                    w[q][1] = kb < a.blocks && second ? __ldg(sw + a.blocks + kb) : 0.f;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) v[q][j] = kb < a.blocks && t0 + 32 * j < a.M ? __ldcg(a.a_scale + (size_t)kb * a.M + t0 + 32 * j) : 0.f;
-                }
-            };
-            ask(0, now, now_w);
-            for (int kb0 = 0; kb0 < a.blocks && ok; kb0 += 4) {
-                ask(kb0 + 4, next, next_w);
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    if (kb0 + q >= a.blocks || !ok) continue;
-                    ok = mbar_wait_warp(SLOT_EMPTY(p), p_round ^ 1, s_abort, a.err);
-                    if (!ok) continue;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) slots[p * 130 + lane + 32 * j] = now[q][j];
-                    if (lane < 2) slots[p * 130 + 128 + lane] = lane ? now_w[q][1] : now_w[q][0];
-                    mbar_arrive_warp(ACC_FULL(p));
-                    if (++p == 2) p = 0, p_round ^= 1;
-                }
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) now[q][j] = next[q][j];
-                    now_w[q][0] = next_w[q][0], now_w[q][1] = next_w[q][1];
-                }
-            }
-        }
-    }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegs));
         const int quarter = warp & 3, half = (warp - 4) / 4;
@@ -328,6 +328,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constan
     // neither CTA leaves while the other's products may read its operands or its barriers be arrived at
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    fp8_settle(s_abort);
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");

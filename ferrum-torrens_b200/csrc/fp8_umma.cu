@@ -238,10 +238,6 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
                 __syncwarp();
             }
         }
-        // given up: the copies in flight land before the CTA leaves
-        if (!ok)
-            for (uint32_t j = asked > (uint32_t)a.stages ? asked - a.stages : 0; j < asked; j++)
-                for (uint32_t i = 0; i < kSpin && !mbar_try_wait(FULL(j % a.stages), (j / a.stages) & 1); i++) {}
     } else if (warp == 1 || warp == 3) {
         // two issuers take the blocks in turn: what a wait and the issue cost one of them passes while the other issues
         Ring st(a.stages), p(S::kAcc);
@@ -400,8 +396,11 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
     if (!left) cluster_arrive();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "n"(S::kTmem) : "memory");
     if (split > 1) cluster_join();
+    if (warp == 2) {
+        fp8_settle(s_abort);
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "n"(S::kTmem) : "memory");
+    }
 }
 
 template <int NT, bool FUSED>
