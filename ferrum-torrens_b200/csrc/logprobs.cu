@@ -476,7 +476,9 @@ logprobs_kernel(LogprobArgs a, int parts) {
         const float bound = from_ordered(s_bound);
         const uint32_t bound_word = W::all(bound);
         for (int g = 0; tiles > 0 && g <= (tiles - 1) >> together; g++) {
-            if (note[warp][g] < s_bound || note[warp][g] == ordered(-kInf)) continue;
+            // (compared as floats: a tile of -0 reaches a bound of 0, one noted as a NaN is read as well)
+            const float most = from_ordered(note[warp][g]);
+            if (most < bound || most == -kInf) continue;
             for (int tile = g << together; tile < min(tiles, (g + 1) << together); tile++) {
                 fetch(tile);
                 uint32_t hit = 0;      // 128-bit words with an element that reaches the bound

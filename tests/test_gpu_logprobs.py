@@ -264,3 +264,16 @@ def test_refusals(moe):
         assert run(**kw) == L.ERR_BAD, kw
     assert lib.ftm_logprobs(null, null, 0, 1, 1, 1, null, 2, 0, null, null, null, null, null, null) == L.ERR_BAD
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("vocab,n", [(5000, 5), (40001, 32), (248320, 20)])
+def test_zeros_of_either_sign_far_apart(moe, vocab, n, dtype):
+    """The two zeros are equal wherever they lie: stretches of one sign that are longer than what any warp reads at a time."""
+    x = torch.zeros((4, vocab), device=DEV, dtype=DT[dtype])
+    x[0, :vocab // 2] = -0.0
+    x[1, vocab // 2:] = -0.0
+    x[2, :vocab - 40] = -0.0
+    x[3, 40:] = -0.0
+    check(moe, x, torch.tensor([vocab // 3, vocab - 1, vocab - 5, 41], device=DEV), n)
+    check(moe, x.repeat(160, 1), torch.tensor([vocab // 3, vocab - 1, vocab - 5, 41], device=DEV).repeat(160), n)
