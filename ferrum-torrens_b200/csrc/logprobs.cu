@@ -377,10 +377,12 @@ logprobs_kernel(LogprobArgs a, int parts) {
     if (tid < 32) best[tid] = 0;
     Stats st;
     int ahead = 0;
+    bool room = true;      // for another candidate (where there is none, this lane stops collecting)
     auto collect = [&](float v, int at, float bound) {
         if (v >= bound && v > -kInf) {
             const int place = atomicAdd(&c_count, 1);
-            if (place < kCandidates) found[place] = key_of(v, at);
+            room = place < kCandidates;
+            if (room) found[place] = key_of(v, at);
         }
     };
     // the elements outside whole words: one per lane of the first CTA's first warp
@@ -475,7 +477,7 @@ logprobs_kernel(LogprobArgs a, int parts) {
         __syncthreads();
         const float bound = from_ordered(s_bound);
         const uint32_t bound_word = W::all(bound);
-        for (int g = 0; tiles > 0 && g <= (tiles - 1) >> together; g++) {
+        for (int g = 0; tiles > 0 && g <= (tiles - 1) >> together && room; g++) {
             // (compared as floats: a tile of -0 reaches a bound of 0, one noted as a NaN is read as well)
             const float most = from_ordered(note[warp][g]);
             if (most < bound || most == -kInf) continue;
@@ -485,11 +487,11 @@ logprobs_kernel(LogprobArgs a, int parts) {
 #pragma unroll
                 for (int u = 0; u < kVecs; u++)
                     hit |= W::any_reaches(W::larger(W::larger(next[u].x, next[u].y), W::larger(next[u].z, next[u].w)), bound_word) ? 1u << u : 0u;
-                for (; hit; hit &= hit - 1) {
+                for (; hit && room; hit &= hit - 1) {
                     const int vi = first_of(tile) + lane + (__ffs(hit) - 1) * 32, at = head + vi * kPer;
                     if (vi >= v1) continue;      // (the fill behind the part's last word reaches a bound of -inf)
                     const uint4 r = __ldg(xv + vi);
-                    for (uint32_t m = W::reaching(r, bound_word); m; m &= m - 1) {
+                    for (uint32_t m = W::reaching(r, bound_word); m && room; m &= m - 1) {
                         const int e = __ffs(m) - 1;
                         collect(load_logit(x + at + e), at + e, bound);
                     }
@@ -507,13 +509,33 @@ logprobs_kernel(LogprobArgs a, int parts) {
                 if (place < n) best[place] = k;
             }
         } else {
+            // Ties: every warp keeps its best as a list.  Its tiles come by index, so once the list is full only what is above its
+            // last entry can enter, and a tile whose maximum is not is left out unread.
             TopList top;
-            for (int vi = v0 + warp * 32; vi < v1; vi += kThreads)
-                for (int e = 0; e < kPer; e++) {
-                    const int at = head + min(vi + lane, v1 - 1) * kPer + e;
-                    const float v = vi + lane < v1 ? load_logit(x + at) : -kInf;
-                    top.offer(v >= bound && v > -kInf ? key_of(v, at) : 0, n, lane);
+            float least = -kInf;      // the list's last value once it is full
+            for (int g = 0; tiles > 0 && g <= (tiles - 1) >> together; g++) {
+                const float most = from_ordered(note[warp][g]);
+                if (most < bound || most <= least) continue;
+                for (int tile = g << together; tile < min(tiles, (g + 1) << together); tile++) {
+                    fetch(tile);
+                    uint32_t hit = 0;      // 128-bit words that any lane has something in
+#pragma unroll
+                    for (int u = 0; u < kVecs; u++) {
+                        const float v = W::largest(W::larger(W::larger(next[u].x, next[u].y), W::larger(next[u].z, next[u].w)));
+                        hit |= v > least && v >= bound ? 1u << u : 0u;
+                    }
+                    for (hit = __reduce_or_sync(0xffffffffu, hit); hit; hit &= hit - 1) {
+                        const int vi = first_of(tile) + lane + (__ffs(hit) - 1) * 32;
+#pragma unroll 1
+                        for (int e = 0; e < kPer; e++) {
+                            const int at = head + vi * kPer + e;
+                            const float v = vi < v1 ? load_logit(x + at) : -kInf;
+                            top.offer(v >= bound && v > -kInf ? key_of(v, at) : 0, n, lane);
+                        }
+                        if (top.last != 0) least = key_value(top.last);
+                    }
                 }
+            }
             top.offer(extra_x >= bound && extra_x > -kInf ? key_of(extra_x, extra_at) : 0, n, lane);
             // (in the place of the candidates; kWarps lists of 32)
             found[tid] = top.k;

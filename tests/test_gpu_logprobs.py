@@ -277,3 +277,44 @@ def test_zeros_of_either_sign_far_apart(moe, vocab, n, dtype):
     x[3, 40:] = -0.0
     check(moe, x, torch.tensor([vocab // 3, vocab - 1, vocab - 5, 41], device=DEV), n)
     check(moe, x.repeat(160, 1), torch.tensor([vocab // 3, vocab - 1, vocab - 5, 41], device=DEV).repeat(160), n)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,vocab,n", [(1, 248320, 20), (3, 40001, 32), (640, 20003, 7), (160, 60000, 20)])
+def test_more_ties_than_candidates(moe, rows, vocab, n, dtype):
+    """Many elements that reach the bound, some tied with it and some above, in stretches, spread out and behind one another."""
+    gen = torch.Generator(device=DEV).manual_seed(rows + vocab)
+    x = torch.full((rows, vocab), torch.finfo(torch.bfloat16).min, device=DEV)
+    steps = torch.arange(vocab, device=DEV)
+    for r in range(min(rows, 160)):
+        kind = r % 8 if rows > 3 else r + 3
+        if kind == 1:
+            x[r, 997::vocab // 5] = 1.0                  # fewer left than alternatives
+        elif kind == 2:
+            x[r, vocab // 3:] = 2.0
+        elif kind == 3:
+            x[r] = (torch.rand(vocab, generator=gen, device=DEV) * 5).floor()
+        elif kind == 4:
+            x[r] = (steps * 64 // vocab).float()
+        elif kind == 5:
+            x[r] = -(steps * 64 // vocab).float()
+            x[r, -3:] = 1.0
+        elif kind == 6:
+            x[r, -700:] = 3.0
+            x[r, -1] = 4.0
+            x[r, ::211] = 3.0
+        elif kind == 7:
+            x[r] = float("nan")
+            x[r, 5::2] = 1.0
+    x[160:] = x[:160].repeat(4, 1)[:max(0, rows - 160)]
+    ids = torch.randint(0, vocab, (rows,), generator=gen, device=DEV)
+    x = x.to(DT[dtype])
+    got = moe.logprobs(x, ids, n)
+    if rows > 160:
+        for t in (got[1], got[3], got[4]):               # (their tokens differ)
+            for i in range(160, rows, 160):
+                assert torch.equal(t[i:i + 160].view(torch.int32), t[:160].view(torch.int32))
+    x, ids = x[:160], ids[:160]
+    want, _, _ = definition(x, ids.cpu().numpy(), n)
+    assert np.array_equal(got[3][:160].cpu().numpy(), want[3]) and np.array_equal(got[2][:160].cpu().numpy(), want[2])
+    check(moe, x, ids, n)
