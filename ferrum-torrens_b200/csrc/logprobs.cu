@@ -19,6 +19,7 @@
 //
 // Rows of small batches are split over the CTAs of a cluster, so that every SM loads; results are sent to the first CTA's shared memory, so no workspace in global memory is needed and calls on
 // several streams share nothing.
+#include <cfloat>
 #include <climits>
 
 #include "kernels.cuh"
@@ -427,8 +428,9 @@ logprobs_kernel(LogprobArgs a, int parts) {
         const int id_vec = want >= head && want < head + vecs * kPer ? (want - head) / kPer : -1;
         if (low_id) {
             // -inf and NaN come behind everything else, by index
+            const uint32_t finite = W::all(-FLT_MAX);
             for (int vi = v0 + tid; vi < v1; vi += kThreads)
-                for (int e = 0; e < kPer; e++) ahead += load_logit(x + head + vi * kPer + e) > -kInf || head + vi * kPer + e < want;
+                ahead += __popc(W::reaching(__ldg(xv + vi), finite) | ((1u << min(max(want - head - vi * kPer, 0), kPer)) - 1));
             if (extra) ahead += extra_x > -kInf || extra_at < want;
         } else if (id_vec >= v0 && id_vec < v1 && tid == 0 && head + id_vec * kPer < want) {
             // the token's own word was counted as in front of it: the token and its equals behind it do not count
