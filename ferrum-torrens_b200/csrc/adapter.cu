@@ -1330,10 +1330,11 @@ FTM_API int ftm_fp8_linear(ftm_handle* h, const void* x, int x_dtype, int64_t x_
     if (rc == FTM_OK) rc = check_fp8_weight(h, "fp8 linear", w_e4m3, w_scale, n, c, c_dtype, c_stride);
     if (rc != FTM_OK) return rc;
     const Ctx ctx = h->ctx(pick(h, stream));
-    if (fp8_fused_supported(m, k))
+    const bool scratch = q_scratch && scale_scratch;
+    if (fp8_fused_supported(m, k) && (!scratch || fp8_fused_faster(m, n, k, h->sm_count)))
         return count_launches(h, launch_fp8_linear(x, x_dtype, x_stride, (const uint8_t*)w_e4m3, w_scale, m, n, k, c, c_dtype, c_stride, h->sm_count,
                                                    h->flags + 2, ctx), "fp8 linear");
-    if (!q_scratch || !scale_scratch) return fail(h, FTM_ERR_BAD, "moe: fp8 linear: %d rows of %d need scratch for their codes and scales", m, k);
+    if (!scratch) return fail(h, FTM_ERR_BAD, "moe: fp8 linear: %d rows of %d need scratch for their codes and scales", m, k);
     rc = check_fp8_codes(h, "fp8 linear", q_scratch, scale_scratch);
     if (rc != FTM_OK) return rc;
     rc = count_launches(h, launch_fp8_quantize(x, x_dtype, m, k, x_stride, (uint8_t*)q_scratch, scale_scratch, h->sm_count, ctx), "fp8 quantize");

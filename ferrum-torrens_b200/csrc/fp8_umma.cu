@@ -496,6 +496,17 @@ int launch(const uint8_t* codes, const uint8_t* w, Fp8Args a, int sm_count, cuda
 // FUSED keeps the codes of sixteen rows in shared memory beside the weight ring
 bool fp8_fused_supported(int M, int K) { return M <= 16 && K <= 8192; }
 
+// In one kernel every CTA quantises all that it multiplies before its first product and keeps the codes; in two that is done once,
+// and the rings are longer.  The second launch costs the host 2.5 us, so two kernels are for where they save the GPU about that:
+// more than 16 blocks of codes to a CTA (fewer than four weight boxes beside them) or more than 160 blocks of one row to quantise.
+// Rows x weight rows x k, us in one and in two kernels of a graph: one is taken for 1 x 248320 x 2048 79.7, 83.3; 8 x 2048 x 4096
+// 6.3, 6.4; 13 x 2048 x 4096 7.4, 6.6; 16 x 2048 x 8192 10.2, 8.2; two for 16 x 248320 x 2048 87.7, 84.9; 16 x 60000 x 2048
+// 29.3, 25.1; 3 x 40000 x 4096 43, 35; 2 x 20000 x 8192 55, 31.
+bool fp8_fused_faster(int M, int N, int K, int sm_count) {
+    const int blocks = (K + kFp8Block - 1) / kFp8Block, split = plan_for<16, true>(M, N, blocks, sm_count).split, mine = (blocks + split - 1) / split;
+    return mine <= 16 && mine * M <= 160;
+}
+
 int launch_fp8_gemm(const uint8_t* a, const float* a_scale, const uint8_t* w, const float* w_scale, int M, int N, int K, void* out,
                     int out_dtype, long long ldc, int sm_count, int32_t* err, const Ctx& c) {
     Fp8Args g{};

@@ -261,8 +261,9 @@ int launch_dense_gemv(const void* a, int a_dtype, const uint32_t* packed, const 
 int launch_fp8_quantize(const void* x, int x_dtype, int rows, int K, long long stride, uint8_t* q, float* scale, int sm_count, const Ctx& c);
 int launch_fp8_gemm(const uint8_t* a, const float* a_scale, const uint8_t* w, const float* w_scale, int M, int N, int K, void* out,
                     int out_dtype, long long ldc, int sm_count, int32_t* err, const Ctx& c);
-// quantisation and product in one kernel
+// quantisation and product in one kernel: where that is possible, and where it is faster than two
 bool fp8_fused_supported(int M, int K);
+bool fp8_fused_faster(int M, int N, int K, int sm_count);
 int launch_fp8_linear(const void* x, int x_dtype, long long x_stride, const uint8_t* w, const float* w_scale, int M, int N, int K, void* out,
                       int out_dtype, long long ldc, int sm_count, int32_t* err, const Ctx& c);
 

@@ -693,14 +693,14 @@ class B200MoE:
         return out
 
     def fp8_linear(self, x, w, w_scale, out, scratch=None, stream=None):
-        """out [M, N] = fp8_gemm of fp8_quantize(x): x [M, K] bf16 or f32 (rows may be apart), the rest as for fp8_gemm.  Up to
-        16 rows of up to 8192 elements are one kernel; above, `scratch` is a pair as fp8_quantize returns it for x, kept
-        by the caller (made here when it is None)."""
+        """out [M, N] = fp8_gemm of fp8_quantize(x): x [M, K] bf16 or f32 (rows may be apart), the rest as for fp8_gemm.
+        `scratch`: a pair as fp8_quantize returns it for x, kept by the caller, for the sizes that are faster in two kernels than
+        in one (made here when it is None and the rows are many or long)."""
         ty = _types()
         px = self._rows(x, "x", ty.act)
         m, n, k, blocks, pw, pws, pc = self._fp8_operands(ty, x, w, w_scale, out)
         on = self._on(stream)
-        if scratch is None and (m > 16 or k > 8192):
+        if scratch is None and (m > 16 or k > 8192 or m * k > 20480 or (k > 2048 and m * k >= 8192)):
             scratch = self._fp8_pair(x, m, k, on)
         pq = ps = None
         if scratch is not None:

@@ -262,7 +262,7 @@ FTM_API int ftm_dense_gemv(ftm_handle* h, const void* a, int a_dtype, const void
  *   a0 = max(largest magnitude of the block, 448 * 2^-126),  scale = a0 / 448,  q = e4m3(x * (448 / a0))
  * in f32, rounded to the nearest code, ties to even; a NaN stays one and does not count as a magnitude, a block with an
  * infinity has scale infinity and codes 0 and NaN.  x [rows, k] bf16 or f32 dev, its rows x_stride elements apart;
- * q [rows, k] e4m3 dev, 16-byte aligned; scale [ceil(k / 128), rows] f32 dev.  k a multiple of 16; rows and k at most 2^30.
+ * q [rows, k] e4m3 dev, 16-byte aligned; scale [ceil(k / 128), rows] f32 dev.  k a multiple of 16; rows and k at least 1, at most 2^30.
  * As in the calls below, outputs overlap no input.  Asynchronous. */
 FTM_API int ftm_fp8_quantize(ftm_handle* h, const void* x, int x_dtype, int32_t rows, int32_t k, int64_t x_stride, void* q_e4m3,
                              float* scale, void* stream);
@@ -270,12 +270,13 @@ FTM_API int ftm_fp8_quantize(ftm_handle* h, const void* x, int x_dtype, int32_t 
  * every sum in f32, c rounded once.  a [m, k] and a_scale as ftm_fp8_quantize writes them; w [n, k] e4m3 dev and w_scale
  * [ceil(n / 128), ceil(k / 128)] f32 dev, the layout of checkpoints in 8 bits; a and w 16-byte aligned.  c [m, n] bf16 or
  * f32 dev, its rows c_stride elements apart (what lies between n and c_stride is not written).  k a multiple of 16; any m
- * and n; each at most 2^30.  The same inputs give the same bits.  Asynchronous. */
+ * and n from 1 on; each at most 2^30.  The same inputs give the same bits.  Asynchronous. */
 FTM_API int ftm_fp8_gemm(ftm_handle* h, const void* a_e4m3, const float* a_scale, const void* w_e4m3, const float* w_scale, int32_t m,
                          int32_t n, int32_t k, void* c, int c_dtype, int64_t c_stride, void* stream);
-/* ftm_fp8_gemm of ftm_fp8_quantize(x) in one call; for up to 16 rows of up to 8192 elements in one kernel, which needs no scratch
- * (both may be NULL).  Above that q_scratch [m, k] (16-byte aligned) and scale_scratch [ceil(k / 128), m] f32 are the caller's,
- * so calls that overlap on the GPU do not meet in them.  Asynchronous. */
+/* ftm_fp8_gemm of ftm_fp8_quantize(x) in one call.  q_scratch [m, k] (16-byte aligned) and scale_scratch [ceil(k / 128), m] f32 are
+ * the caller's, so calls that overlap on the GPU do not meet in them.  Up to 16 rows of up to 8192 elements can be one kernel,
+ * which needs neither: they may be NULL then; given both, the call takes what is faster (many rows or long ones: two kernels).
+ * The bits are the same.  Asynchronous. */
 FTM_API int ftm_fp8_linear(ftm_handle* h, const void* x, int x_dtype, int64_t x_stride, const void* w_e4m3, const float* w_scale,
                            int32_t m, int32_t n, int32_t k, void* q_scratch, float* scale_scratch, void* c, int c_dtype,
                            int64_t c_stride, void* stream);

@@ -186,6 +186,23 @@ def test_linear_is_the_product_of_the_quantised_rows(moe, m, n, k, pad, offset, 
     moe.sync_status()
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 40000, 2048), (2, 20000, 8192), (4, 10240, 8192), (5, 2048, 8192), (8, 2048, 4096), (12, 100, 2048), (13, 2048, 4096), (16, 8192, 512),
+                                   (16, 1000, 8192), (16, 60000, 1040)])
+def test_one_kernel_and_two_give_the_same_bits(moe, m, n, k):
+    x = activations(m + n, m, k, torch.bfloat16).contiguous()
+    w, ws = weight(n + k, n, k)
+    c = torch.full((3, m, n), 77.0, device=DEV)
+    scratch = moe.fp8_quantize(torch.zeros_like(x))
+    lib, p, st = L.lib(), lambda t: C.c_void_p(t.data_ptr()), C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    call = lambda q, s, out: lib.ftm_fp8_linear(moe._h, p(x), L.BF16, k, p(w), p(ws), m, n, k, q, s, p(out), L.F32, n, st)
+    assert call(C.c_void_p(0), C.c_void_p(0), c[0]) == L.OK
+    assert call(p(scratch[0]), p(scratch[1]), c[1]) == L.OK
+    moe.fp8_gemm(*moe.fp8_quantize(x), w, ws, c[2])
+    assert torch.equal(c[0], c[1]) and torch.equal(c[0], c[2])
+    check_product(c[0], *quantised(x), w, ws)
+    moe.sync_status()
+
+
 @pytest.mark.parametrize("sms", [1, 2, 7, 40])
 @pytest.mark.parametrize("m", [3, 30, 50, 120, 300, 700])
 def test_few_sms(moe, m, sms):
