@@ -107,11 +107,11 @@ struct Fp8Args {
 
 template <int NT, bool FUSED>
 struct Shape {
-    static constexpr int kEpi = NT >= 64 ? 8 : 4;                // epilogue warps
+    static constexpr int kEpi = NT >= 128 ? 16 : NT >= 64 ? 8 : 4;      // epilogue warps
     static constexpr int kHelp = FUSED ? 4 : 0;                  // more warps that quantise
     static constexpr int kThreads = 128 + 32 * (kEpi + kHelp);
     static constexpr int kCols = NT * 4 / kEpi;                  // columns of one epilogue warp
-    static constexpr int kAcc = NT >= 128 ? 2 : 4;               // accumulators (and slots of scales)
+    static constexpr int kAcc = 4;                               // accumulators (and slots of scales)
     static constexpr int kTmem = NT * kAcc < 32 ? 32 : NT * kAcc;
     static constexpr int kABytes = NT * kFp8Block;               // a token box
     static constexpr int kPerSm = NT <= 32 ? 2 : 1;              // CTAs of an SM
