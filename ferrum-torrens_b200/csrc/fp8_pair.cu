@@ -43,7 +43,8 @@ struct PairArgs {
     int M, N, blocks;
     int m_tiles, tiles;
     void* c;
-    int c_dtype, c_align;        // c_align: 16, 8, 4 or 2, what every row of c is aligned to (16: stored by TMA)
+    int c_dtype;
+    bool c_by_tma, c_by_8;       // every row of c starts on 16 bytes, on 8
     long long ldc;
     int32_t* err;
 };
@@ -87,7 +88,7 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
 // One warp's 32 tokens from t0 on by 256 bytes of output from weight row n0 on, from its (swizzled) place in shared memory to c.
 __device__ __forceinline__ void send_out(const PairArgs& a, const CUtensorMap* map, uint8_t* from, int t0, int n0, int elem, int lane) {
     const int cols = 128 / elem;      // of a box
-    if (a.c_align == 16) {
+    if (a.c_by_tma) {
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) {
@@ -100,20 +101,34 @@ __device__ __forceinline__ void send_out(const PairArgs& a, const CUtensorMap* m
         }
         return;
     }
-    // rows that are less aligned: lanes side by side along a row, as many bytes each as the alignment allows
+    // Other rows: a lane has 8 bytes of each.  Where not all rows start on 8 bytes, these are moved up by the neighbour's so that they do in
+    // memory.  What is left at the rows' two ends then goes out in pieces of 2, a row to a lane.
     __syncwarp();
-    const int log_piece = a.c_align == 8 ? 3 : a.c_align == 4 ? 2 : 1, log_elem = elem == 2 ? 1 : 2, piece = 1 << log_piece;
-#pragma unroll 4
-    for (int i = 0; i < 256 >> log_piece; i++) {      // 32 pieces each time
-        const int at = (i * 32 << log_piece) + (lane << log_piece), row = at >> 8, byte = at & 255, col = n0 + (byte >> log_elem);
-        if (t0 + row >= a.M || col >= a.N) continue;
-        const uint8_t* const src = from + (byte >> 7) * 4096 + row * 128 + ((((byte >> 4) & 7) ^ (row & 7)) << 4) + (byte & 15);
-        uint8_t* const dst = reinterpret_cast<uint8_t*>(a.c) + (((t0 + row) * a.ldc + col) << log_elem);
-        const int bytes = min(piece, (a.N - col) << log_elem);
-        if (bytes == 8) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(src);
-        else if (bytes == 4) *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
-        else
-            for (int b = 0; b < bytes; b += 2) *reinterpret_cast<uint16_t*>(dst + b) = *reinterpret_cast<const uint16_t*>(src + b);
+    const int rows = min(32, a.M - t0), bytes = min(256, (a.N - n0) * elem);
+    const long long next = a.ldc * elem;
+    uint8_t* const first = reinterpret_cast<uint8_t*>(a.c) + ((long long)t0 * a.ldc + n0) * elem;
+    auto at = [&](int row, int byte) { return from + (byte >> 7) * 4096 + row * 128 + ((((byte >> 4) & 7) ^ (row & 7)) << 4) + (byte & 15); };
+    if (a.c_by_8) {
+        if (8 * lane + 8 <= bytes)
+#pragma unroll 8
+            for (int row = 0; row < rows; row++) *reinterpret_cast<uint64_t*>(first + row * next + 8 * lane) = *reinterpret_cast<const uint64_t*>(at(row, 8 * lane));
+    } else {
+#pragma unroll 8
+        for (int row = 0; row < rows; row++) {
+            uint8_t* const to = first + row * next;
+            const uint64_t cur = *reinterpret_cast<const uint64_t*>(at(row, 8 * lane)), before = __shfl_up_sync(0xffffffffu, cur, 1);
+            const int off = (int)(reinterpret_cast<uintptr_t>(to) & 7), byte = 8 * lane - off;
+            if (byte >= 0 && byte + 8 <= bytes) *reinterpret_cast<uint64_t*>(to + byte) = off ? cur << (8 * off) | before >> (64 - 8 * off) : cur;
+        }
+    }
+    if (lane < rows) {
+        uint8_t* const to = first + lane * next;
+        const int ahead = min((int)(-reinterpret_cast<uintptr_t>(to) & 7), bytes), behind = ahead + ((bytes - ahead) & ~7);
+#pragma unroll
+        for (int q = 0; q < 6; q += 2) {
+            if (q < ahead) *reinterpret_cast<uint16_t*>(to + q) = *reinterpret_cast<const uint16_t*>(at(lane, q));
+            if (behind + q < bytes) *reinterpret_cast<uint16_t*>(to + behind + q) = *reinterpret_cast<const uint16_t*>(at(lane, behind + q));
+        }
     }
     __syncwarp();
 }
@@ -358,11 +373,12 @@ int launch_fp8_pair(const uint8_t* a, const float* a_scale, const uint8_t* w, co
     g.tiles = g.m_tiles * ((N + kN - 1) / kN);
     g.c = out; g.c_dtype = out_dtype; g.ldc = ldc; g.err = err;
     const int elem = out_dtype == 0 ? 2 : 4;
-    g.c_align = 16;
-    while (g.c_align > elem && (reinterpret_cast<uintptr_t>(out) % g.c_align || ldc * elem % g.c_align)) g.c_align /= 2;
+    const uint64_t starts = reinterpret_cast<uintptr_t>(out) | (uint64_t)(ldc * elem);
+    g.c_by_tma = starts % 16 == 0;
+    g.c_by_8 = starts % 8 == 0;
     CUtensorMap map_a, map_w, map_c{};
     if (!fp8_codes_map(&map_a, a, M, K, 128) || !fp8_codes_map(&map_w, w, N, K, 128)) return -(int)cudaErrorInvalidValue;
-    if (g.c_align == 16 && !out_map(&map_c, out, out_dtype, M, N, ldc)) return -(int)cudaErrorInvalidValue;
+    if (g.c_by_tma && !out_map(&map_c, out, out_dtype, M, N, ldc)) return -(int)cudaErrorInvalidValue;
     static PerDeviceOnce once;
     cudaError_t e = allow_dyn_smem(once, fp8_pair_kernel, kSmem);
     if (e != cudaSuccess) return -(int)e;

@@ -240,6 +240,62 @@ def test_output_rows_of_any_alignment(moe, n, ld, offset, out):
     assert (buf[kept] == 77.0).all()
 
 
+@pytest.fixture(params=[0, 20])
+def sms(request, moe):
+    """All SMs, or so few that many rows are taken by pairs of them in tiles of 256 x 256."""
+    moe.set_sm_budget(request.param)
+    yield request.param
+    moe.set_sm_budget(0)
+
+
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+@pytest.mark.parametrize("n,ld,offset", [(1281, 1281, 0), (1407, 1407, 1), (1409, 1411, 0), (1534, 1534, 0), (1535, 1537, 3), (1539, 1540, 2), (1343, 1346, 0), (1280, 1284, 4)])
+def test_rows_that_start_and_end_anywhere(moe, sms, n, ld, offset, out):
+    """Outputs of odd sizes, with ends of every length."""
+    m, k = 1100, 128
+    q, s = moe.fp8_quantize(activations(n, m, k, torch.bfloat16))
+    w, ws = weight(ld, n, k)
+    buf = torch.full((m * ld + offset + 9,), 77.0, dtype=DT[out], device=DEV)
+    c = buf.as_strided((m, n), (ld, 1), storage_offset=offset)
+    moe.fp8_gemm(q, s, w, ws, c)
+    check_product(c, q.double().cpu().numpy(), s.cpu().numpy(), w, ws)
+    kept = torch.ones_like(buf, dtype=torch.bool)
+    kept.as_strided((m, n), (ld, 1), storage_offset=offset).fill_(False)
+    assert (buf[kept] == 77.0).all()
+    moe.sync_status()
+
+
+@pytest.mark.parametrize("m,n,k", [(1000, 4100, 2000), (1025, 4097, 272), (600, 9000, 1040), (4097, 1025, 640), (257, 20000, 144)])
+def test_pairs_of_sms(moe, sms, m, n, k):
+    q, s = moe.fp8_quantize(activations(m + n, m, k, torch.float32))
+    w, ws = weight(k + n, n, k)
+    for out in (torch.bfloat16, torch.float32):
+        c = torch.full((m + 1, n), 77.0, dtype=out, device=DEV)
+        moe.fp8_gemm(q, s, w, ws, c[:m])
+        check_product(c[:m], q.double().cpu().numpy(), s.cpu().numpy(), w, ws)
+        assert (c[m] == 77.0).all()
+    moe.sync_status()
+
+
+@pytest.mark.parametrize("m", [300, 1100])
+def test_special_codes_in_tiles_of_pairs(moe, sms, m):
+    """A NaN code is its weight row's matter, an infinite scale its token's."""
+    n, k = 1400, 400
+    q, s = moe.fp8_quantize(activations(3, m, k, torch.bfloat16))
+    w, ws = weight(4, n, k)
+    clean = torch.empty((m, n), device=DEV)
+    moe.fp8_gemm(q, s, w, ws, clean)
+    wb, s2 = w.clone().view(torch.uint8), s.clone()
+    wb[1333, 399], s2[1, m // 2] = 0x7f, float("inf")
+    got = torch.empty_like(clean)
+    moe.fp8_gemm(q, s2, wb.view(E4M3), ws, got)
+    got, clean = got.cpu().numpy(), clean.cpu().numpy()
+    assert np.isnan(got[:, 1333]).all() and not np.isfinite(got[m // 2]).any()
+    rows, cols = np.arange(m) != m // 2, np.arange(n) != 1333
+    assert np.array_equal(got[np.ix_(rows, cols)], clean[np.ix_(rows, cols)])
+    moe.sync_status()
+
+
 @pytest.mark.parametrize("m", [1, 9, 40, 130, 600])
 def test_special_codes_stay_in_their_row_or_column(moe, m):
     n, k = 300, 400
