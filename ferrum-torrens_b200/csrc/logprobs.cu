@@ -331,7 +331,7 @@ logprobs_kernel(LogprobArgs a, int parts) {
     __shared__ float p_stat[kWarps][3];           // m, s, t
     __shared__ int p_rank[kWarps];
     __shared__ int note[kWarps][kNotes];          // (ordered) maxima of a warp's part of one or more tiles
-    __shared__ __align__(16) int lane_max[kThreads];       // (ordered)
+    __shared__ int lane_max[kThreads];            // (ordered)
 
     // whole 128-bit words of the row, and the elements in front of and behind them
     const int head = min((int)(((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / sizeof(T)), a.vocab);
@@ -457,13 +457,13 @@ logprobs_kernel(LogprobArgs a, int parts) {
     }
     if (n > 0) {
         if (warp == 0) {
-            // the n-th largest of 64 values, each the largest of some lanes' maxima, two to a lane here
-            constexpr int kHalf = kThreads / 64;
+            // the n-th largest of 64 values, each the largest of some lanes' maxima (of every 64th lane: in a short row one warp may have
+            // all the elements), two to a lane here
             int u = INT_MIN, w = INT_MIN;
 #pragma unroll
-            for (int q = 0; q < kHalf; q++) {
-                u = max(u, lane_max[lane * kHalf + q]);
-                w = max(w, lane_max[kThreads / 2 + lane * kHalf + q]);
+            for (int q = 0; q < kThreads; q += 64) {
+                u = max(u, lane_max[q + lane]);
+                w = max(w, lane_max[q + 32 + lane]);
             }
             int best = INT_MIN;
 #pragma unroll 1
