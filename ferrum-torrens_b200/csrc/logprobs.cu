@@ -101,6 +101,10 @@ struct Word<float> {
         return any_reaches(w.x, v) | any_reaches(w.y, v) << 1 | any_reaches(w.z, v) << 2 | any_reaches(w.w, v) << 3;
     }
     // how many elements of four words are above v, added to a tile's counts of even and odd elements
+    // elements of a word that are v become -inf and are counted, in each half of `taken`
+    __device__ __forceinline__ static void take_out(uint32_t& w, uint32_t v, uint32_t& taken) {
+        if (__uint_as_float(w) == __uint_as_float(v)) w = kLowest, taken++;
+    }
     using Count = uint64_t;
     __device__ __forceinline__ static float above(uint32_t w, float v) {
         float r;
@@ -140,6 +144,11 @@ struct Word<__nv_bfloat16> {
         const uint32_t m = a | b | c | d;
         return (m | m >> 16) & 0xffu;
     }
+    __device__ __forceinline__ static void take_out(uint32_t& w, uint32_t v, uint32_t& taken) {
+        const uint32_t same = __heq2_mask(as2(w), as2(v));
+        w = (w & ~same) | (kLowest & same);
+        taken += same & 0x10001u;
+    }
     using Count = __nv_bfloat162;      // (a tile's counts of even and odd elements are whole numbers that a bf16 holds)
     __device__ __forceinline__ static void count_above(const uint4& w, uint32_t v, __nv_bfloat162& count) {
         count = __hadd2(count, __hadd2(__hadd2(__hgt2(as2(w.x), as2(v)), __hgt2(as2(w.y), as2(v))), __hadd2(__hgt2(as2(w.z), as2(v)), __hgt2(as2(w.w), as2(v)))));
@@ -152,20 +161,22 @@ struct Word<__nv_bfloat16> {
     }
 };
 
-// softmax statistics of what was read: the maximum, the sum of the exponentials and that of e^d d
+// Softmax statistics of what was read: the maximum, the sum of the exponentials and that of e^d d.  The elements that made the
+// maximum rise are counted in `ones` and left out of s: beside their 1 a small s would lose its last places, and the logarithm
+// of a sum close to 1 (a token that is all but certain) with them.
 struct Stats {
     float m = -kInf, s = 0.f, t = 0.f;
+    int ones = 0;
 
     // distance from the maximum `top` that this one is joined under: 0 where nothing was summed (or a NaN, which stays)
     __device__ __forceinline__ float below(float top) const { return m == -kInf ? 0.f : max_nan(m - top, kFar); }
-    // the maximum may rise to mx.  (The lanes of a warp share theirs, so that the branch is taken by all or none.)
+    // the maximum rises to mx (the lanes of a warp share theirs)
     __device__ __forceinline__ void rise(float mx) {
-        if (mx > m) {
-            const float d = below(mx), f = ex2(d * kLog2e);
-            t = f * (t + s * d);
-            s *= f;
-            m = mx;
-        }
+        const float d = below(mx), f = ex2(d * kLog2e), all = s + (float)ones;
+        t = f * (t + all * d);
+        s = f * all;
+        ones = 0;
+        m = mx;
     }
     // the elements of one 128-bit word; s2 and t2 hold sums of even and odd elements until take()
     template <typename T>
@@ -197,15 +208,13 @@ struct Stats {
     // the lanes' statistics joined, in every lane
     __device__ __forceinline__ void join_warp() {
         const float top = from_ordered(__reduce_max_sync(0xffffffffu, ordered(m)));
-        const float d = below(top), f = ex2(d * kLog2e);
-        t = f * (t + s * d);
-        s *= f;
-        m = top;
+        if (!(m == top)) rise(top);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             s += __shfl_xor_sync(0xffffffffu, s, o);
             t += __shfl_xor_sync(0xffffffffu, t, o);
         }
+        ones = __reduce_add_sync(0xffffffffu, ones);
     }
 };
 
@@ -324,12 +333,12 @@ logprobs_kernel(LogprobArgs a, int parts) {
 
     __shared__ __align__(8) uint64_t arrived;     // first CTA: counts the bytes the others send
     __shared__ uint64_t lists[kMaxCluster][32];   // first CTA: the best of every CTA of the cluster
-    __shared__ uint32_t c_all[kMaxCluster][4];    // first CTA: m, s, t and rank of every CTA
+    __shared__ uint32_t c_all[kMaxCluster][5];    // first CTA: m, s, t, rank and ones of every CTA
     __shared__ uint64_t best[32];                 // this CTA's best
     __shared__ __align__(16) uint64_t found[kCandidates];  // elements that reached the bound
     __shared__ int c_count, s_bound;
     __shared__ float p_stat[kWarps][3];           // m, s, t
-    __shared__ int p_rank[kWarps];
+    __shared__ int p_rank[kWarps], p_ones[kWarps];
     __shared__ int note[kWarps][kNotes];          // (ordered) maxima of a warp's part of one or more tiles
     __shared__ int lane_max[kThreads];            // (ordered)
 
@@ -357,7 +366,7 @@ logprobs_kernel(LogprobArgs a, int parts) {
             const uint32_t bar = shared_addr(&arrived);
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar));
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-            if (part == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"((parts - 1) * (4 + 2 * n) * 4) : "memory");
+            if (part == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"((parts - 1) * (5 + 2 * n) * 4) : "memory");
         }
         __syncwarp();
         asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
@@ -393,8 +402,9 @@ logprobs_kernel(LogprobArgs a, int parts) {
     float lane_m = fmaxf(extra_x, -kInf);      // (a NaN is not a maximum)
     if (extra && asked && !low_id) ahead += extra_x > (extra_at < want ? x_id_below : x_id);
     if (part == 0 && warp == 0) {
-        st.rise(from_ordered(__reduce_max_sync(0xffffffffu, ordered(lane_m))));
-        if (extra) st.add_one(extra_x);
+        st.m = from_ordered(__reduce_max_sync(0xffffffffu, ordered(lane_m)));
+        if (extra && extra_x == st.m && st.m > -kInf) st.ones = 1;
+        else if (extra) st.add_one(extra_x);
     }
     __syncwarp();
 
@@ -412,17 +422,25 @@ logprobs_kernel(LogprobArgs a, int parts) {
         lane_m = fmaxf(lane_m, mx);
         const int warp_mx = __reduce_max_sync(0xffffffffu, ordered(mx));
         if (lane == 0) note[warp][tile >> together] = together ? max(note[warp][tile >> together], warp_mx) : warp_mx;
-        st.rise(from_ordered(warp_mx));
-        uint64_t s2 = 0, t2 = 0;
-#pragma unroll
-        for (int u = 0; u < kVecs; u++) st.template add<T>(r[u], s2, t2);
-        st.take(s2, t2);
         if (mx >= look) {
             typename W::Count count = W::none();
 #pragma unroll
             for (int u = 0; u < kVecs; u++) W::count_above(r[u], head + (first_of(tile) + lane + u * 32) * kPer < want ? below_word : id_word, count);
             ahead += W::total(count);
         }
+        const float risen = from_ordered(warp_mx);
+        if (risen > st.m) {
+            st.rise(risen);
+            const uint32_t out = W::all(risen);
+            uint32_t taken = 0;
+#pragma unroll
+            for (int u = 0; u < kVecs; u++) W::take_out(r[u].x, out, taken), W::take_out(r[u].y, out, taken), W::take_out(r[u].z, out, taken), W::take_out(r[u].w, out, taken);
+            st.ones = (int)((taken & 0xffffu) + (taken >> 16));
+        }
+        uint64_t s2 = 0, t2 = 0;
+#pragma unroll
+        for (int u = 0; u < kVecs; u++) st.template add<T>(r[u], s2, t2);
+        st.take(s2, t2);
     }
     if (asked) {
         const int id_vec = want >= head && want < head + vecs * kPer ? (want - head) / kPer : -1;
@@ -442,17 +460,17 @@ logprobs_kernel(LogprobArgs a, int parts) {
     lane_max[tid] = ordered(lane_m);
     st.join_warp();
     ahead = __reduce_add_sync(0xffffffffu, ahead);
-    if (lane == 0) p_stat[warp][0] = st.m, p_stat[warp][1] = st.s, p_stat[warp][2] = st.t, p_rank[warp] = ahead;
+    if (lane == 0) p_stat[warp][0] = st.m, p_stat[warp][1] = st.s, p_stat[warp][2] = st.t, p_rank[warp] = ahead, p_ones[warp] = st.ones;
     __syncthreads();
     if (warp == kWarps - 1) {
         Stats all;
         int sum = 0;
-        if (lane < kWarps) all.m = p_stat[lane][0], all.s = p_stat[lane][1], all.t = p_stat[lane][2], sum = p_rank[lane];
+        if (lane < kWarps) all.m = p_stat[lane][0], all.s = p_stat[lane][1], all.t = p_stat[lane][2], all.ones = p_ones[lane], sum = p_rank[lane];
         all.join_warp();
         sum = __reduce_add_sync(0xffffffffu, sum);
         if (lane == 0) {
             c_all[part][0] = __float_as_uint(all.m), c_all[part][1] = __float_as_uint(all.s), c_all[part][2] = __float_as_uint(all.t);
-            c_all[part][3] = (uint32_t)sum;
+            c_all[part][3] = (uint32_t)sum, c_all[part][4] = (uint32_t)all.ones;
         }
     }
     if (n > 0) {
@@ -557,7 +575,7 @@ logprobs_kernel(LogprobArgs a, int parts) {
         const uint32_t bar = shared_addr(&arrived);
         if (part != 0) {
             const uint32_t to = in_first_cta(bar);
-            if (lane < 4) send(in_first_cta(shared_addr(&c_all[part][lane])), c_all[part][lane], to);
+            if (lane < 5) send(in_first_cta(shared_addr(&c_all[part][lane])), c_all[part][lane], to);
             if (lane < n) {
                 const uint32_t at = in_first_cta(shared_addr(&lists[part][lane]));
                 send(at, (uint32_t)best[lane], to);
@@ -577,15 +595,15 @@ logprobs_kernel(LogprobArgs a, int parts) {
     int rank = 0;
     if (lane < parts) {
         all.m = __uint_as_float(c_all[lane][0]), all.s = __uint_as_float(c_all[lane][1]), all.t = __uint_as_float(c_all[lane][2]);
-        rank = (int)c_all[lane][3];
+        rank = (int)c_all[lane][3], all.ones = (int)c_all[lane][4];
     }
     all.join_warp();
     rank = __reduce_add_sync(0xffffffffu, rank);
 
     // ---- results ------------------------------------------------------------------------------------
-    const float m = all.m, total = all.s, t = all.t;
-    const bool broken = total != total, empty = !broken && m == -kInf;
-    const float log_s = empty ? 0.f : logf(total);
+    const float m = all.m, rest = all.s + (float)(all.ones - 1), total = all.s + (float)all.ones, t = all.t;
+    const bool broken = total != total || m == kInf, empty = !broken && m == -kInf;
+    const float log_s = empty ? 0.f : log1pf(rest);
     const float nan = __int_as_float(0x7fffffff);
     auto prob = [&](float v) { return broken ? nan : empty ? -kInf : (v - m) - log_s; };
     if (lane == 0) {

@@ -318,3 +318,28 @@ def test_more_ties_than_candidates(moe, rows, vocab, n, dtype):
     want, _, _ = definition(x, ids.cpu().numpy(), n)
     assert np.array_equal(got[3][:160].cpu().numpy(), want[3]) and np.array_equal(got[2][:160].cpu().numpy(), want[2])
     check(moe, x, ids, n)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,vocab", [(3, 700), (700, 1500), (5, 40001), (1, 248320), (300, 70000)])
+def test_tokens_that_are_all_but_certain(moe, rows, vocab, dtype):
+    """The log probability of such a token, and its row's entropy, to the precision of their own small values."""
+    x = logits_of(rows, rows, vocab, DT[dtype])
+    x = x.clamp(max=14)
+    gen = torch.Generator(device=DEV).manual_seed(vocab)
+    ids = torch.randint(0, vocab, (rows,), generator=gen, device=DEV)
+    ids[0] = vocab - 1
+    x[torch.arange(rows, device=DEV), ids] = torch.tensor([22.0, 28.0, 20.0, 34.0, 25.0], device=DEV).repeat(rows)[:rows].to(DT[dtype])
+    got = moe.logprobs(x, ids, 1)
+    d = x.double() - x.double().amax(-1, keepdim=True)
+    e = d.exp()
+    e[torch.arange(rows, device=DEV), ids] = 0.0
+    rest = e.sum(-1)
+    dist = -(e * torch.where(e > 0, d, 0.0)).sum(-1)
+    lp, ent = -torch.log1p(rest), torch.log1p(rest) + dist / (1 + rest)
+    # of the rest's sum: vocab / 256 + 40 additions, exponentials within 2^-21, their arguments (up to 60) off by their own size times 2^-23
+    tol = (vocab / 256 + 40) * 2.0 ** -24 + 2.0 ** -21 + 60 * 2.0 ** -22
+    assert ((got[0].double() - lp).abs() <= tol * lp.abs()).all()
+    assert torch.equal(got[4][:, 0], got[0])
+    assert ((got[1].double() - ent).abs() <= 2 * tol * ent).all()
+    assert (got[2] == 0).all() and torch.equal(got[3][:, 0].long(), ids)
