@@ -137,12 +137,13 @@ struct ftm_handle {
 namespace {
 
 // Makes the adapter's device current for one call and restores the caller's on the way out: a host
-// thread that drives adapters on several devices need not switch devices itself.
+// thread that drives adapters on several devices need not switch devices itself.  The device is set where it is current already,
+// too: in a thread that has not used CUDA yet that is what binds its context, which encoding a tensor map needs.
 struct DeviceGuard {
     int prev = -1;
     bool switched = false;
     explicit DeviceGuard(int want) {
-        if (cudaGetDevice(&prev) == cudaSuccess && prev != want) switched = cudaSetDevice(want) == cudaSuccess;
+        if (cudaGetDevice(&prev) == cudaSuccess) switched = cudaSetDevice(want) == cudaSuccess && prev != want;
     }
     ~DeviceGuard() {
         if (switched) cudaSetDevice(prev);

@@ -462,3 +462,76 @@ def test_refusals(moe):
         assert linear(**kw) == L.ERR_BAD, kw
     assert lib.ftm_fp8_gemm(null, null, null, null, null, 1, 1, 16, null, 0, 1, null) == L.ERR_BAD
     torch.cuda.synchronize()
+
+
+def test_calls_from_several_threads(moe):
+    """Kernels of every kind beside one another, from host threads with a stream each, give what they give alone."""
+    import threading
+    gen = rng(11)
+    pk = torch.randint(-2 ** 31, 2 ** 31 - 1, (128, 4096), generator=gen, device=DEV, dtype=torch.int32)
+    sk = torch.randint(0x20, 0x40, (64, 4096), generator=gen, device=DEV, dtype=torch.uint8)
+    glob = torch.full((4096,), 0x3c00, device=DEV, dtype=torch.int16)
+    act = activations(5, 64, 1024, torch.bfloat16).contiguous()
+    logits, ids = activations(6, 40, 30001, torch.float32), torch.arange(40, device=DEV)
+    jobs = []
+    for i, (m, n, k) in enumerate([(1000, 4100, 2000), (100, 4096, 2048), (13, 2048, 4096), (64, 10240, 512), (1500, 2000, 1024), (30, 3000, 2048)]):
+        x, (w, ws) = activations(i, m, k, torch.bfloat16).contiguous(), weight(i + 1, n, k)
+        scratch = moe.fp8_quantize(x)
+
+        def linear(stream, x=x, w=w, ws=ws, scratch=scratch, c=torch.empty((m, n), device=DEV)):
+            return [moe.fp8_linear(x, w, ws, c, scratch=scratch, stream=stream)]
+        jobs.append(linear)
+    out = moe.logprobs(logits, ids, 9)
+    jobs.append(lambda stream: list(moe.logprobs(logits, ids, 9, out=out, stream=stream)))
+    c = torch.empty((64, 4096), device=DEV)
+    jobs.append(lambda stream: [moe.dense_gemv(act, pk, sk, glob, c, stream=stream)])
+    alone = []
+    for job in jobs:
+        alone.append([t.clone() for t in job(torch.cuda.current_stream())])
+    torch.cuda.synchronize()
+    failures = []
+
+    def work(job, want):
+        stream = torch.cuda.Stream(device=0)
+        try:
+            for _ in range(5):
+                for _ in range(20):
+                    got = job(stream)
+                stream.synchronize()
+                for a, b in zip(got, want):
+                    if not torch.equal(a.view(torch.int32), b.view(torch.int32)):
+                        failures.append("another result")
+        except Exception as e:
+            failures.append(repr(e))
+    threads = [threading.Thread(target=work, args=a) for a in zip(jobs, alone)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures, failures
+    moe.sync_status()
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 600, 1024), (40, 600, 1024), (1000, 4100, 2000)])
+def test_first_call_of_a_host_thread(moe, m, n, k):
+    """A thread in which nothing has used CUDA yet."""
+    import threading
+    x, (w, ws) = activations(1, m, k, torch.bfloat16).contiguous(), weight(2, n, k)
+    q, s = moe.fp8_quantize(x)
+    want, c = torch.empty((m, n), device=DEV), torch.zeros((2, m, n), device=DEV)
+    moe.fp8_gemm(q, s, w, ws, want)
+    stream = torch.cuda.current_stream().cuda_stream
+    torch.cuda.synchronize()
+    lib, p, st, null = L.lib(), lambda t: C.c_void_p(t.data_ptr()), C.c_void_p(stream), C.c_void_p(0)
+    codes, args = [], [(p(q), p(s), p(w), p(ws), p(c[0])), (p(x), p(w), p(ws), p(c[1]))]
+    calls = [lambda: codes.append(lib.ftm_fp8_gemm(moe._h, *args[0][:4], m, n, k, args[0][4], L.F32, n, st))]
+    if m <= 16:
+        calls.append(lambda: codes.append(lib.ftm_fp8_linear(moe._h, args[1][0], L.BF16, k, args[1][1], args[1][2], m, n, k, null, null, args[1][3], L.F32, n, st)))
+    for call in calls:
+        t = threading.Thread(target=call)
+        t.start()
+        t.join()
+    torch.cuda.synchronize()
+    assert codes == [L.OK] * len(calls)
+    for i in range(len(calls)):
+        assert torch.equal(c[i], want)
