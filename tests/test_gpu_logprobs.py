@@ -343,3 +343,26 @@ def test_tokens_that_are_all_but_certain(moe, rows, vocab, dtype):
     assert torch.equal(got[4][:, 0], got[0])
     assert ((got[1].double() - ent).abs() <= 2 * tol * ent).all()
     assert (got[2] == 0).all() and torch.equal(got[3][:, 0].long(), ids)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_the_largest_vocabularies(moe, dtype):
+    """Parts of more tiles than there are notes: one row of 2^24, and rows of 600001 that have a CTA each."""
+    x = logits_of(1, 1, 2 ** 24, DT[dtype])
+    check(moe, x, torch.tensor([2 ** 24 - 5], device=DEV), 32)
+    x[0, 5::1000] = 30.0                                 # more ties than candidates
+    check(moe, x, torch.tensor([2 ** 23 + 5], device=DEV), 20)
+    del x
+    rows, vocab, n = 650, 600001, 20
+    x = logits_of(2, rows, vocab, DT[dtype])
+    x[1, ::3] = 20.0
+    x[2] = torch.arange(vocab, device=DEV).float() / 1024
+    ids = torch.randint(0, vocab, (rows,), generator=torch.Generator(device=DEV).manual_seed(1), device=DEV)
+    got = moe.logprobs(x, ids, n)
+    some = [0, 1, 2, 300, rows - 1]
+    want, tol, tol_ent = definition(x[some], ids[some].cpu().numpy(), n)
+    assert np.array_equal(got[3][some].cpu().numpy(), want[3]) and np.array_equal(got[2][some].cpu().numpy(), want[2])
+    close(got[0][some], want[0], tol)
+    close(got[1][some], want[1], tol_ent)
+    close(got[4][some], want[4], tol)
+    moe.sync_status()
