@@ -36,9 +36,10 @@ namespace {
 constexpr int kMaxCluster = 16;      // more than 8 CTAs need the opt-in of launch_logprobs
 constexpr int kVecs = 4;             // 128-bit words of a lane per tile
 constexpr int kWarpVecs = 32 * kVecs;        // 128-bit words of a warp per tile
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kInf = __builtin_huge_valf();
 constexpr float kFar = -1e20f;       // differences below this have exponential 0; clamped there, sums of them stay finite
+constexpr float kLarge = 1e30f;      // maxima below this in magnitude: products with log2(e) stay finite
 constexpr int kCandidates = 512;
 constexpr int kNotes = 64;           // noted maxima of a warp; longer parts note several tiles together
 constexpr uint32_t kSpin = 1u << 24; // looks at a barrier before a wait is given up (a part full of ties takes some ms longer than the others)
@@ -106,6 +107,8 @@ struct Word<float> {
         return any_reaches(w.x, v) | any_reaches(w.y, v) << 1 | any_reaches(w.z, v) << 2 | any_reaches(w.w, v) << 3;
     }
     // how many elements of four words are above v, added to a tile's counts of even and odd elements
+    __device__ __forceinline__ static uint64_t both(uint32_t w) { return w; }      // (these two are for words of two elements)
+    __device__ __forceinline__ static uint32_t at_least(uint32_t w, uint32_t) { return w; }
     // elements of a word that are v become -inf and are counted, in each half of `taken`
     __device__ __forceinline__ static void take_out(uint32_t& w, uint32_t v, uint32_t& taken) {
         if (__uint_as_float(w) == __uint_as_float(v)) w = kLowest, taken++;
@@ -149,6 +152,12 @@ struct Word<__nv_bfloat16> {
         const uint32_t m = a | b | c | d;
         return (m | m >> 16) & 0xffu;
     }
+    __device__ __forceinline__ static uint64_t both(uint32_t w) { return pair(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+    // the larger of each, or a NaN where w is one
+    __device__ __forceinline__ static uint32_t at_least(uint32_t w, uint32_t v) {
+        const __nv_bfloat162 r = __hmax2_nan(as2(w), as2(v));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
     __device__ __forceinline__ static void take_out(uint32_t& w, uint32_t v, uint32_t& taken) {
         const uint32_t same = __heq2_mask(as2(w), as2(v));
         w = (w & ~same) | (kLowest & same);
@@ -166,49 +175,76 @@ struct Word<__nv_bfloat16> {
     }
 };
 
-// Softmax statistics of what was read: the maximum, the sum of the exponentials and that of e^d d.  The elements that made the
-// maximum rise are counted in `ones` and left out of s: beside their 1 a small s would lose its last places, and the logarithm
-// of a sum close to 1 (a token that is all but certain) with them.
+// Softmax statistics of what was read: the maximum m, the sum of the exponentials and that of e^d d, in powers of two:
+//   z = x log2(e) - c,  s = sum 2^z,  t = sum 2^z z      c = m log2(e) rounded to a whole number
+// so that z is one multiply-add, and a tile whose maximum rises less than that changes nothing.  (Where m is too large for that, z is
+// (x - m) log2(e).)  The elements that made the maximum rise are counted in `ones` and left out of s: beside them a small s would lose its
+// last places, and the logarithm of a sum close to one element (a token that is all but certain) with them.
 struct Stats {
     float m = -kInf, s = 0.f, t = 0.f;
     int ones = 0;
 
-    // distance from the maximum `top` that this one is joined under: 0 where nothing was summed (or a NaN, which stays)
-    __device__ __forceinline__ float below(float top) const { return m == -kInf ? 0.f : max_nan(m - top, kFar); }
+    __device__ __forceinline__ bool near() const { return fabsf(m) < kLarge; }
+    __device__ __forceinline__ float whole() const { return rintf(m * kLog2e); }
+    // z of the maximum
+    __device__ __forceinline__ float own() const { return near() ? fmaf(m, kLog2e, -whole()) : 0.f; }
     // the maximum rises to mx (the lanes of a warp share theirs)
     __device__ __forceinline__ void rise(float mx) {
-        const float d = below(mx), f = ex2(d * kLog2e), all = s + (float)ones;
-        t = f * (t + all * d);
+        const float from = m, z = own(), e = (float)ones * ex2(z), all = s + e;
+        m = mx;
+        const float d = (from == -kInf ? 0.f : max_nan((from - mx) * kLog2e, kFar)) + (own() - z), f = ex2(d);
+        t = f * (fmaf(e, z, t) + all * d);
         s = f * all;
         ones = 0;
-        m = mx;
     }
-    // the elements of one 128-bit word; s2 and t2 hold sums of even and odd elements until take()
+    __device__ __forceinline__ static void add_two(uint64_t z, uint64_t& s2, uint64_t& t2) {
+        const float2 v = unpair(z);
+        const uint64_t e = pair(ex2(v.x), ex2(v.y));
+        s2 = add2(s2, e);
+        t2 = fma2(e, z, t2);
+    }
+    __device__ __forceinline__ static uint64_t clamped(uint64_t z) {
+        const float2 v = unpair(z);
+        return pair(max_nan(v.x, kFar), max_nan(v.y, kFar));
+    }
+    // the elements of one tile
     template <typename T>
-    __device__ __forceinline__ void add(const uint4& v, uint64_t& s2, uint64_t& t2) const {
-        const float from = m == -kInf ? 0.f : -m;
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    __device__ __forceinline__ void add(const uint4 (&r)[kVecs]) {
+        using W = Word<T>;
+        uint64_t s2 = 0, t2 = 0;
+        if (near()) {
+            const uint64_t c = pair(-whole(), -whole()), by = pair(kLog2e, kLog2e);
+            // what is this far below m has exponential 0 (and -inf times 0 would be a NaN)
+            const uint32_t lowest = W::all(m - fmaxf(200.f, fabsf(m) * 0.03125f));
 #pragma unroll
-        for (int j = 0; j < 4; j += 2 / Word<T>::kElems) {
-            const uint64_t x = Word<T>::kElems == 2 ? pair(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u))
-                                                    : pair(__uint_as_float(w[j]), __uint_as_float(w[(j + 1) & 3]));
-            const float2 y = unpair(add2(x, pair(from, from)));
-            const uint64_t d = pair(max_nan(y.x, kFar), max_nan(y.y, kFar));
-            const float2 z = unpair(mul2(d, pair(kLog2e, kLog2e)));
-            const uint64_t e = pair(ex2(z.x), ex2(z.y));
-            s2 = add2(s2, e);
-            t2 = fma2(e, d, t2);
+            for (int u = 0; u < kVecs; u++) {
+                const uint32_t w[4] = {r[u].x, r[u].y, r[u].z, r[u].w};
+#pragma unroll
+                for (int j = 0; j < 4; j += 2 / W::kElems) {
+                    if (W::kElems == 2) add_two(fma2(W::both(W::at_least(w[j], lowest)), by, c), s2, t2);
+                    else add_two(clamped(fma2(pair(__uint_as_float(w[j]), __uint_as_float(w[(j + 1) & 3])), by, c)), s2, t2);
+                }
+            }
+        } else {
+            const float from = m == -kInf ? 0.f : -m;
+#pragma unroll
+            for (int u = 0; u < kVecs; u++) {
+                const uint32_t w[4] = {r[u].x, r[u].y, r[u].z, r[u].w};
+#pragma unroll
+                for (int j = 0; j < 4; j += 2 / W::kElems) {
+                    const uint64_t x = W::kElems == 2 ? W::both(w[j]) : pair(__uint_as_float(w[j]), __uint_as_float(w[(j + 1) & 3]));
+                    add_two(mul2(clamped(add2(x, pair(from, from))), pair(kLog2e, kLog2e)), s2, t2);
+                }
+            }
         }
-    }
-    __device__ __forceinline__ void take(uint64_t s2, uint64_t t2) {
         const float2 a = unpair(s2), b = unpair(t2);
         s += a.x + a.y;
         t += b.x + b.y;
     }
     __device__ __forceinline__ void add_one(float x) {
-        const float d = max_nan(x - (m == -kInf ? 0.f : m), kFar), e = ex2(d * kLog2e);
+        const float z = max_nan(near() ? fmaf(x, kLog2e, -whole()) : (x - (m == -kInf ? 0.f : m)) * kLog2e, kFar), e = ex2(z);
         s += e;
-        t = fmaf(e, d, t);
+        t = fmaf(e, z, t);
     }
     // the lanes' statistics joined, in every lane
     __device__ __forceinline__ void join_warp() {
@@ -442,10 +478,7 @@ logprobs_kernel(LogprobArgs a, int parts) {
             for (int u = 0; u < kVecs; u++) W::take_out(r[u].x, out, taken), W::take_out(r[u].y, out, taken), W::take_out(r[u].z, out, taken), W::take_out(r[u].w, out, taken);
             st.ones = (int)((taken & 0xffffu) + (taken >> 16));
         }
-        uint64_t s2 = 0, t2 = 0;
-#pragma unroll
-        for (int u = 0; u < kVecs; u++) st.template add<T>(r[u], s2, t2);
-        st.take(s2, t2);
+        st.template add<T>(r);
     }
     if (asked) {
         const int id_vec = want >= head && want < head + vecs * kPer ? (want - head) / kPer : -1;
@@ -606,7 +639,9 @@ logprobs_kernel(LogprobArgs a, int parts) {
     rank = __reduce_add_sync(0xffffffffu, rank);
 
     // ---- results ------------------------------------------------------------------------------------
-    const float m = all.m, rest = all.s + (float)(all.ones - 1), total = all.s + (float)all.ones, t = all.t;
+    // in units of the maximum's own exponential, and of e
+    const float m = all.m, z = all.own(), unit = ex2(-z), sum = all.s * unit, t = (all.t - z * all.s) * unit * kLn2;
+    const float rest = sum + (float)(all.ones - 1), total = sum + (float)all.ones;
     const bool broken = total != total || m == kInf, empty = !broken && m == -kInf;
     const float log_s = empty ? 0.f : log1pf(rest);
     const float nan = __int_as_float(0x7fffffff);
