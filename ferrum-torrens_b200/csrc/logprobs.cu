@@ -5,9 +5,9 @@
 //   logprob = d_id - log s,   entropy = log s - t / s,
 //   rank = #{v : x_v > x_id, or x_v = x_id and v < id},   alternatives in the order (value descending, index ascending)
 //
-// Every thread keeps m, s and t of what it has read in f32 (pairs of elements in one instruction) and rescales s and t when its
-// maximum rises (t gains s * (old - new)); the partial triples are joined over the warp, the CTA and the cluster.
-// Differences are clamped at -1e20: an element of -inf adds e^d = 0 times a finite d; NaN and +inf make s a NaN.
+// Every thread keeps s and t of what it has read in f32 (pairs of elements in one instruction), and rescales them when its warp's
+// maximum rises (t gains s * (old - new)); the partial sums are joined over the warp, the CTA and the cluster.
+// Differences are clamped: an element of -inf adds e^d = 0 times a finite d; a NaN makes s a NaN.
 //
 // Alternatives (n <= 32).  The pass itself only notes the maximum of every warp's part of every tile.  The lanes' maxima, some
 // taken together, give 64 values, and the n-th largest of these is a bound: n elements reach it, so what is below
@@ -20,8 +20,8 @@
 // Rows of small batches are split over the CTAs of a cluster, so that every SM loads; results are sent to the first CTA's shared
 // memory, so no workspace in global memory is needed and calls on several streams share nothing.
 //
-// Bound by instruction issue and the exponentials' unit where there are rows for all SMs (999 x 248320 bf16, one alternative: 108 us,
-// 4600 GB/s, 0.71 of measured HBM; 512 x 248320 f32 5600 GB/s; 4096 x 32003 bf16, 20 alternatives: 83 us), by the passage from the last
+// Bound by instruction issue and the exponentials' unit where there are rows for all SMs (999 x 248320 bf16, one alternative: 104 us,
+// 4760 GB/s, 0.74 of measured HBM; 512 x 248320 f32 5600 GB/s; 4096 x 32003 bf16, 20 alternatives: 81 us), by the passage from the last
 // load to the results, about 5 us, in single waves (64 x 248320 f32, 5 alternatives: 18 us; one row, 20 alternatives: 10 us).  Through
 // a ring in shared memory filled by bulk copies the same rows took 176 and 109 us.
 #include <cfloat>
@@ -711,7 +711,7 @@ int launch_logprobs(const void* logits, int dtype, int rows, int vocab, long lon
     LogprobArgs a{logits, stride, vocab, ids, ids_dtype, top_n, logprob, entropy, rank, top_ids, top_logprobs, bad_flag, err};
     const int elem = dtype == 0 ? 2 : 4;
     // Eight warps to a CTA; four where there are many rows that are short, for more of them at a time and less to join (4096 rows of
-    // 32003 bf16: 79 us against 89; 999 rows of 248320 bf16: 117 against 109)
+    // 32003 bf16: 79 us against 89; 999 rows of 248320 bf16: 117 against 109, both before small sums kept their places)
     const bool narrow = rows > 4 * sm_count && (long long)vocab * elem <= 8 * 8 * kWarpVecs * 16;
     // CTAs per row: as many as keep every SM at 32 warps (clusters of more than eight CTAs do not pack that well: up to one per SM),
     // each with two tiles of its own at least
