@@ -46,7 +46,7 @@ struct PairArgs {
     int m_tiles, tiles;
     void* c;
     int c_dtype;
-    bool c_by_tma, c_by_8;       // every row of c starts on 16 bytes, on 8
+    bool c_by_tma, c_by_8;       // every row of c starts and ends on 16 bytes, starts on 8
     long long ldc;
     int32_t* err;
 };
@@ -376,7 +376,8 @@ int launch_fp8_pair(const uint8_t* a, const float* a_scale, const uint8_t* w, co
     g.c = out; g.c_dtype = out_dtype; g.ldc = ldc; g.err = err;
     const int elem = out_dtype == 0 ? 2 : 4;
     const uint64_t starts = reinterpret_cast<uintptr_t>(out) | (uint64_t)(ldc * elem);
-    g.c_by_tma = starts % 16 == 0;
+    // (a row that ends within 16 bytes: the copy would write them whole, though the map ends with the row)
+    g.c_by_tma = starts % 16 == 0 && (int64_t)N * elem % 16 == 0;
     g.c_by_8 = starts % 8 == 0;
     CUtensorMap map_a, map_w, map_c{};
     if (!fp8_codes_map(&map_a, a, M, K, 128) || !fp8_codes_map(&map_w, w, N, K, 128)) return -(int)cudaErrorInvalidValue;

@@ -535,3 +535,42 @@ def test_first_call_of_a_host_thread(moe, m, n, k):
     assert codes == [L.OK] * len(calls)
     for i in range(len(calls)):
         assert torch.equal(c[i], want)
+
+
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+@pytest.mark.parametrize("m,n,k", [(33, 300, 1040), (65, 257, 2048), (40, 9001, 1040), (60, 4099, 4112), (65, 2050, 8192), (100, 1000, 8192), (90, 8191, 2064),
+                                   (100, 4097, 4112), (130, 2051, 8208), (500, 2000, 4112), (300, 4100, 400), (250, 4100, 1040)])
+def test_tiles_of_every_width_whole_and_split(moe, m, n, k, out):
+    """Tiles of 32, 64 and 128 tokens, each with a CTA of its own and with several that share its blocks."""
+    q, s = moe.fp8_quantize(activations(m + n, m, k, torch.float32))
+    w, ws = weight(k + n, n, k)
+    buf = torch.full((m + 1, n + 3), 77.0, dtype=DT[out], device=DEV)
+    c = buf[:m, :n]
+    moe.fp8_gemm(q, s, w, ws, c)
+    check_product(c, q.double().cpu().numpy(), s.cpu().numpy(), w, ws)
+    assert (buf[:, n:] == 77.0).all() and (buf[m] == 77.0).all()
+    again = torch.empty((m, n), dtype=DT[out], device=DEV)
+    moe.fp8_gemm(q, s, w, ws, again)
+    assert torch.equal(again, c)
+    moe.sync_status()
+
+
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+@pytest.mark.parametrize("n,ld,offset", [(1281, 1281, 0), (1407, 1407, 1), (1409, 1411, 0), (1534, 1534, 0), (1535, 1537, 3), (1539, 1540, 2), (1343, 1346, 0), (1280, 1284, 4),
+                                         (1300, 1304, 8)])
+def test_rows_of_pairs_start_and_end_anywhere(moe, n, ld, offset, out):
+    m, k = 1100, 640
+    q, s = moe.fp8_quantize(activations(n, m, k, torch.bfloat16))
+    w, ws = weight(ld, n, k)
+    buf = torch.full((m * ld + offset + 9,), 77.0, dtype=DT[out], device=DEV)
+    c = buf.as_strided((m, n), (ld, 1), storage_offset=offset)
+    moe.set_sm_budget(10)
+    try:
+        moe.fp8_gemm(q, s, w, ws, c)
+        check_product(c, q.double().cpu().numpy(), s.cpu().numpy(), w, ws)
+        moe.sync_status()
+    finally:
+        moe.set_sm_budget(0)
+    kept = torch.ones_like(buf, dtype=torch.bool)
+    kept.as_strided((m, n), (ld, 1), storage_offset=offset).fill_(False)
+    assert (buf[kept] == 77.0).all()
