@@ -21,6 +21,7 @@
 // over), and by launch and set-up, about 4.5 us, in small calls: 1 x 8192 x 2048 7.2 us, 13 x 2048 x 4096 f32 7.4, 64 x 10240 x 2048 8.2.
 // Every wait is bounded; a wait that gives up raises the error flag and the CTA drains.
 #include <atomic>
+#include <climits>
 #include <type_traits>
 
 #include "fp8.cuh"
@@ -439,20 +440,32 @@ int clusters_at_once(int q) {
     return max(n, 1);
 }
 
-// CTAs that share a tile's blocks, and what a call then waits for, in blocks of one CTA
+// CTAs that share a tile's blocks, and what the call then takes by measurement, in ns: its start, the blocks of the busiest SM (of a
+// CTA alone there or of several) and the join of a cluster's sums.  (Joins of 6 or 12 blocks of time in the place of 9 for NT = 128: no
+// difference over 26 sizes.)
 struct Plan {
-    int split, cost;
+    int split;
+    long long ns;
 };
+struct Costs {
+    int start, alone, several, join, second;      // second: what a second CTA on an SM adds once
+};
+template <int NT>
+constexpr Costs kCosts = NT == 16   ? Costs{2200, 300, 300, 1800, 0}
+                         : NT == 32 ? Costs{2200, 325, 210, 1900, 1000}
+                         : NT == 64 ? Costs{2660, 345, 345, 2070, 0}
+                                    : Costs{3400, 410, 410, 3000, 0};
 template <int NT, bool FUSED>
 Plan plan_for(int M, int N, int blocks, int sm_count) {
     using S = Shape<NT, FUSED>;
+    constexpr Costs c = kCosts<NT>;
     const long long tiles = (long long)((M + NT - 1) / NT) * ((N + kRows - 1) / kRows);
-    const int join = NT <= 64 ? 6 : 9;      // what joining the sums costs, in blocks (13 or more were slower at 2048 rows, fewer at 8192)
-    Plan best{1, (int)min((tiles + sm_count - 1) / sm_count * blocks, 1ll << 30)};
-    for (int q = 2; q <= kMaxSplit && q <= blocks && tiles * q <= S::kPerSm * sm_count; q++) {
-        if (tiles > clusters_at_once<NT, FUSED>(q)) continue;
-        const int cost = (int)((tiles * q + sm_count - 1) / sm_count) * ((blocks + q - 1) / q) + join;
-        if (cost < best.cost) best = {q, cost};
+    Plan best{1, 0};
+    for (int q = 1; q <= kMaxSplit && q <= blocks && (q == 1 || tiles * q <= S::kPerSm * sm_count); q++) {
+        if (q > 1 && tiles > clusters_at_once<NT, FUSED>(q)) continue;
+        const long long each = (tiles * q + sm_count - 1) / sm_count, mine = (blocks + q - 1) / q;
+        const long long ns = c.start + mine * (each > 1 ? c.several * each : c.alone) + (q > 1 ? c.join : 0) + (each > 1 ? c.second : 0);
+        if (q == 1 || ns < best.ns) best = {q, ns};
     }
     return best;
 }
@@ -516,18 +529,24 @@ int launch_fp8_gemm(const uint8_t* a, const float* a_scale, const uint8_t* w, co
     g.a_scale = a_scale; g.w_scale = w_scale; g.M = M; g.N = N; g.K = K; g.c = out; g.c_dtype = out_dtype; g.ldc = ldc; g.err = err;
     c.begin(K_FP8_GEMM);
     int n;
-    // Pairs of SMs where their tiles take less time: a block of 256 x 256 takes 9 / 8 of what one of 128 x 128 takes here.  Us with pairs and
-    // here: 300 x 16384 x 4096 36.4, 44.2; 400 x 5000 x 2048 13.0, 16.9; 1000 x 4100 x 2000 14.4, 18.0; 700 x 2048 x 4096 19.3, 16.6;
-    // 256 x 8192 x 2048 12.8, 9.9; 128 x 16384 x 2048 14.4, 11.3.
     const int blocks = (K + kFp8Block - 1) / kFp8Block;
-    const long long pair_tiles = (long long)((M + 255) / 256) * ((N + 255) / 256), pair_cost = (pair_tiles + sm_count / 2 - 1) / max(1, sm_count / 2) * blocks * 9 / 8;
-    if (M > 128 && sm_count > 1 && pair_cost < plan_for<128, false>(M, N, blocks, sm_count).cost)
-        n = launch_fp8_pair(a, a_scale, w, w_scale, M, N, K, out, out_dtype, ldc, sm_count, err, c.s);
-    else
-        n = M <= 16   ? launch<16, false>(a, w, g, sm_count, c.s)
-            : M <= 32 ? launch<32, false>(a, w, g, sm_count, c.s)
-            : M <= 64 ? launch<64, false>(a, w, g, sm_count, c.s)
-                      : launch<128, false>(a, w, g, sm_count, c.s);
+    if (M <= 16) n = launch<16, false>(a, w, g, sm_count, c.s);
+    else if (M <= 32) n = launch<32, false>(a, w, g, sm_count, c.s);
+    else {
+        // Tiles of 32, 64 or 128 tokens, or pairs of SMs on 256, whichever takes the least time: narrow tiles keep more SMs at work on
+        // small problems, wide ones fetch less.  Us with 32, 64, 128 and pairs: 64 x 512 x 2048 3.9, 4.6, -, -; 512 x 512 x 512 3.6, 3.8, 4.7, -;
+        // 100 x 8192 x 2048 9.5, 8.2, 9.8, -; 512 x 2048 x 2048 9.5, 8.2, 9.7, -; 200 x 8192 x 8192 52.5, 46.9, 29.9, 34.5; 256 x 8192 x 2048
+        // 15.8, 14.1, 9.9, 12.8; 700 x 2048 x 4096 -, -, 16.6, 19.3; 400 x 5000 x 2048 -, -, 16.9, 13.0; 1000 x 8192 x 8192 177, 158, -, 68.
+        const long long pair_tiles = (long long)((M + 255) / 256) * ((N + 255) / 256), pairs = sm_count / 2;
+        const long long ns32 = plan_for<32, false>(M, N, blocks, sm_count).ns, ns64 = plan_for<64, false>(M, N, blocks, sm_count).ns;
+        const long long ns128 = M > 64 ? plan_for<128, false>(M, N, blocks, sm_count).ns : LLONG_MAX;
+        const long long ns_pair = M > 128 && pairs > 0 ? 6000 + 480 * blocks * ((pair_tiles + pairs - 1) / pairs) : LLONG_MAX;
+        const long long least = min(min(ns32, ns64), min(ns128, ns_pair));
+        n = least == ns_pair ? launch_fp8_pair(a, a_scale, w, w_scale, M, N, K, out, out_dtype, ldc, sm_count, err, c.s)
+            : least == ns128 ? launch<128, false>(a, w, g, sm_count, c.s)
+            : least == ns64  ? launch<64, false>(a, w, g, sm_count, c.s)
+                             : launch<32, false>(a, w, g, sm_count, c.s);
+    }
     c.end();
     return n;
 }
