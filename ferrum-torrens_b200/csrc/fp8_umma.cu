@@ -415,10 +415,9 @@ cudaError_t prepare() {
 
 // Clusters of q CTAs that the device holds at a time (SMs are grouped, so eights and sevens leave some of them empty)
 template <int NT, bool FUSED>
-int clusters_at_once(int q) {
+int clusters_at_once(int dev, int q) {
     static std::atomic<int> known[64][kMaxSplit + 1];
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return 0;
+    if (dev < 0 || dev >= 64) return 0;
     int n = known[dev][q].load(std::memory_order_relaxed);
     if (n) return n;
     if (prepare<NT, FUSED>() != cudaSuccess) return 0;
@@ -461,8 +460,10 @@ Plan plan_for(int M, int N, int blocks, int sm_count) {
     constexpr Costs c = kCosts<NT>;
     const long long tiles = (long long)((M + NT - 1) / NT) * ((N + kRows - 1) / kRows);
     Plan best{1, 0};
+    int dev = -1;
+    if (tiles * 2 <= S::kPerSm * sm_count && cudaGetDevice(&dev) != cudaSuccess) dev = -1;
     for (int q = 1; q <= kMaxSplit && q <= blocks && (q == 1 || tiles * q <= S::kPerSm * sm_count); q++) {
-        if (q > 1 && tiles > clusters_at_once<NT, FUSED>(q)) continue;
+        if (q > 1 && tiles > clusters_at_once<NT, FUSED>(dev, q)) continue;
         const long long each = (tiles * q + sm_count - 1) / sm_count, mine = (blocks + q - 1) / q;
         const long long ns = c.start + mine * (each > 1 ? c.several * each : c.alone) + (q > 1 ? c.join : 0) + (each > 1 ? c.second : 0);
         if (q == 1 || ns < best.ns) best = {q, ns};

@@ -722,11 +722,12 @@ class B200MoE:
 
     def _fp8_operands(self, ty, a, w, w_scale, out):
         """Sizes and addresses that fp8_gemm and fp8_linear have in common."""
-        if a.dim() != 2 or w.dim() != 2 or a.shape[1] != w.shape[1]:
-            raise bad(f"fp8: a weight [N, K] is wanted for rows [M, K], got {tuple(w.shape)} for {tuple(a.shape)}")
-        n, k = w.shape
-        m, blocks = a.shape[0], -(-k // 128)
-        return (m, n, k, blocks, self._flat(w, "the weight", ty.e4m3, (n, k)), self._flat(w_scale, "the weight's scales", ty.f32, (-(-n // 128), blocks)),
+        rows, weight = a.shape, w.shape
+        if len(rows) != 2 or len(weight) != 2 or rows[1] != weight[1]:
+            raise bad(f"fp8: a weight [N, K] is wanted for rows [M, K], got {tuple(weight)} for {tuple(rows)}")
+        (m, k), n = rows, weight[0]
+        blocks = -(-k // 128)
+        return (m, n, k, blocks, self._flat(w, "the weight", ty.e4m3, weight), self._flat(w_scale, "the weight's scales", ty.f32, (-(-n // 128), blocks)),
                 self._rows(out, "the output", ty.act, (m, n)))
 
     # -- what a server reads off its logits -----------------------------------------------------
