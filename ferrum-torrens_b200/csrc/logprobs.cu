@@ -107,8 +107,6 @@ struct Word<float> {
         return any_reaches(w.x, v) | any_reaches(w.y, v) << 1 | any_reaches(w.z, v) << 2 | any_reaches(w.w, v) << 3;
     }
     // how many elements of four words are above v, added to a tile's counts of even and odd elements
-    __device__ __forceinline__ static uint64_t both(uint32_t w) { return w; }      // (these two are for words of two elements)
-    __device__ __forceinline__ static uint32_t at_least(uint32_t w, uint32_t) { return w; }
     // elements of a word that are v become -inf and are counted, in each half of `taken`
     __device__ __forceinline__ static void take_out(uint32_t& w, uint32_t v, uint32_t& taken) {
         if (__uint_as_float(w) == __uint_as_float(v)) w = kLowest, taken++;
@@ -221,8 +219,8 @@ struct Stats {
                 const uint32_t w[4] = {r[u].x, r[u].y, r[u].z, r[u].w};
 #pragma unroll
                 for (int j = 0; j < 4; j += 2 / W::kElems) {
-                    if (W::kElems == 2) add_two(fma2(W::both(W::at_least(w[j], lowest)), by, c), s2, t2);
-                    else add_two(clamped(fma2(pair(__uint_as_float(w[j]), __uint_as_float(w[(j + 1) & 3])), by, c)), s2, t2);
+                    if constexpr (W::kElems == 2) add_two(fma2(W::both(W::at_least(w[j], lowest)), by, c), s2, t2);
+                    else add_two(clamped(fma2(pair(__uint_as_float(w[j]), __uint_as_float(w[j + 1])), by, c)), s2, t2);
                 }
             }
         } else {
@@ -232,7 +230,9 @@ struct Stats {
                 const uint32_t w[4] = {r[u].x, r[u].y, r[u].z, r[u].w};
 #pragma unroll
                 for (int j = 0; j < 4; j += 2 / W::kElems) {
-                    const uint64_t x = W::kElems == 2 ? W::both(w[j]) : pair(__uint_as_float(w[j]), __uint_as_float(w[(j + 1) & 3]));
+                    uint64_t x;
+                    if constexpr (W::kElems == 2) x = W::both(w[j]);
+                    else x = pair(__uint_as_float(w[j]), __uint_as_float(w[j + 1]));
                     add_two(mul2(clamped(add2(x, pair(from, from))), pair(kLog2e, kLog2e)), s2, t2);
                 }
             }
