@@ -713,11 +713,19 @@ int launch_logprobs(const void* logits, int dtype, int rows, int vocab, long lon
     // Eight warps to a CTA; four where there are many rows that are short, for more of them at a time and less to join (4096 rows of
     // 32003 bf16: 79 us against 89; 999 rows of 248320 bf16: 117 against 109, both before small sums kept their places)
     const bool narrow = rows > 4 * sm_count && (long long)vocab * elem <= 8 * 8 * kWarpVecs * 16;
-    // CTAs per row: as many as keep every SM at 32 warps (clusters of more than eight CTAs do not pack that well: up to one per SM),
-    // each with two tiles of its own at least
-    const long long tiles = ((long long)vocab * elem + (narrow ? 4 : 8) * kWarpVecs * 16 - 1) / ((narrow ? 4 : 8) * kWarpVecs * 16);
+    // CTAs per row: as many as keep every SM at 32 warps (clusters of more than eight CTAs do not pack that well: up to one per SM), each
+    // with two tiles of its own at least, or with one where it has its SM alone and few alternatives to find.  One row of 248320 f32 with 1, 4,
+    // 8 and 16 CTAs: 34.5, 13.3, 9.5, 7.5 us; 64 of them with 2, 4, 8, 12: 29, 21, 20, 27; 300 of 32003 bf16 with 1, 2, 4: 12, 14, 17.
+    // Parts of one tile in the place of two: 1 x 17000 f32, 8 alternatives, 5.8 us against 7.3; 32 alternatives of 17000 bf16 9.9, 9.4;
+    // 100 x 9000 f32 6.5, 5.9.
+    const int tile_bytes = (narrow ? 4 : 8) * kWarpVecs * 16;
+    const long long tiles = ((long long)vocab * elem + tile_bytes - 1) / tile_bytes;
     int parts = 1;
-    while (parts < kMaxCluster && (long long)rows * (parts + 1) <= (parts < 8 ? (narrow ? 8 : 4) * sm_count : sm_count) && tiles >= 2 * (parts + 1)) parts++;
+    for (int next = 2; next <= kMaxCluster; next++) {
+        const long long ctas = (long long)rows * next;
+        if (ctas > (next <= 8 ? (narrow ? 8 : 4) * sm_count : sm_count) || tiles < next * (top_n <= 16 && ctas <= sm_count ? 1 : 2)) break;
+        parts = next;
+    }
     c.begin(K_LOGPROBS);
     const cudaError_t e = dtype == 0 ? (narrow ? launch<__nv_bfloat16, 4>(a, rows, parts, c.s) : launch<__nv_bfloat16, 8>(a, rows, parts, c.s))
                                      : (narrow ? launch<float, 4>(a, rows, parts, c.s) : launch<float, 8>(a, rows, parts, c.s));
