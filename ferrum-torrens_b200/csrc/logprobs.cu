@@ -39,7 +39,7 @@ constexpr int kWarpVecs = 32 * kVecs;        // 128-bit words of a warp per tile
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kInf = __builtin_huge_valf();
 constexpr float kFar = -1e20f;       // differences below this have exponential 0; clamped there, sums of them stay finite
-constexpr float kLarge = 1e30f;      // maxima below this in magnitude: products with log2(e) stay finite
+constexpr float kLarge = 4e6f;       // maxima below this in magnitude: products with log2(e) are below 2^23, so f32 has the whole number next to them
 constexpr int kCandidates = 512;
 constexpr int kNotes = 64;           // noted maxima of a warp; longer parts note several tiles together
 constexpr uint32_t kSpin = 1u << 24; // looks at a barrier before a wait is given up (a part full of ties takes some ms longer than the others)
@@ -175,8 +175,8 @@ struct Word<__nv_bfloat16> {
 
 // Softmax statistics of what was read: the maximum m, the sum of the exponentials and that of e^d d, in powers of two:
 //   z = x log2(e) - c,  s = sum 2^z,  t = sum 2^z z      c = m log2(e) rounded to a whole number
-// so that z is one multiply-add, and a tile whose maximum rises less than that changes nothing.  (Where m is too large for that, z is
-// (x - m) log2(e).)  The elements that made the maximum rise are counted in `ones` and left out of s: beside them a small s would lose its
+// so that z is one multiply-add, and a tile whose maximum rises less than that changes nothing.  (Where m is so large that c, the rounded
+// product, would be far from m log2(e), z is (x - m) log2(e).)  The elements that made the maximum rise are counted in `ones` and left out of s: beside them a small s would lose its
 // last places, and the logarithm of a sum close to one element (a token that is all but certain) with them.
 struct Stats {
     float m = -kInf, s = 0.f, t = 0.f;

@@ -366,3 +366,45 @@ def test_the_largest_vocabularies(moe, dtype):
     close(got[1][some], want[1], tol_ent)
     close(got[4][some], want[4], tol)
     moe.sync_status()
+
+
+FAR = [s * m for m in (3.9e6, 4.1e6, 1e8, 3e9, 5e9, 1e10, 1e12, 1e20, 9e29) for s in (1.0, -1.0)]
+
+
+def far_rows(vocab):
+    """Finite rows whose maxima lie anywhere between the usual logits and the type's limits, and masks of such values."""
+    g = torch.Generator().manual_seed(vocab)
+    rnd = lambda: torch.randn(vocab, generator=g) * 3
+    rows = []
+    for far in FAR:
+        rows.append(torch.full((vocab,), far))
+        rows.append(rnd() + far)                                           # as close as the type's steps are there
+        rows.append(far + abs(far) * 0.1 * rnd())
+        if far > 0:
+            r = rnd(); r[vocab // 3] = far; rows.append(r)                 # the maximum rises to it
+        else:
+            r = rnd(); r[torch.rand(vocab, generator=g) < 0.9] = far; rows.append(r)
+            r = torch.full((vocab,), far); r[-3:] = rnd()[-3:]; rows.append(r)         # first tiles with nothing else
+            r = torch.full((vocab,), far); r[::2] = -INF; r[vocab // 2] = far * 0.5; rows.append(r)
+    return torch.stack(rows)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("vocab,n,times", [(37, 5, 1), (700, 3, 10), (9000, 20, 9), (70001, 20, 1), (70001, 5, 9)])
+def test_rows_far_from_zero(moe, vocab, n, times, dtype):
+    """Whole rows and, with `times` of each, rows enough for a CTA of eight or of four warps each."""
+    x = far_rows(vocab).to(DT[dtype]).to(DEV)
+    ids = torch.randint(0, vocab, (x.shape[0],), generator=torch.Generator().manual_seed(n)).to(DEV)
+    ids[::2] = x.float().argmax(-1)[::2]
+    want, tol, tol_ent = definition(x, ids.cpu().numpy(), n)
+    # x log2(e) - c is held in f32 where |x| < 4e6, with |c - x log2(e)| < 0.75: within the arguments' 2^-23 and the exponentials' 2^-21
+    tile = lambda v: np.tile(v, (times,) + (1,) * (v.ndim - 1))
+    got = moe.logprobs(x.repeat(times, 1), ids.repeat(times), n)
+    assert np.array_equal(got[3].cpu().numpy(), tile(want[3])) and np.array_equal(got[2].cpu().numpy(), tile(want[2]))
+    close(got[0], tile(want[0]), tile(tol))
+    close(got[1], tile(want[1]), tile(tol_ent))
+    close(got[4], tile(want[4]), tile(tol))
+    if times == 1:
+        for r in range(x.shape[0]):
+            check(moe, x[r:r + 1], ids[r:r + 1], n)
+    moe.sync_status()
