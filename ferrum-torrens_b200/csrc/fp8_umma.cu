@@ -37,6 +37,12 @@ using namespace umma;
 constexpr int kRows = 128;                       // weight rows of a tile
 constexpr int kWBytes = kRows * kFp8Block;       // a weight box
 constexpr int kMaxStages = 12, kMaxAcc = 4, kMaxSplit = 8;
+// The issuers take the blocks in turn.  One that waits for block b has to know that the box a ring before has come, or it may take that
+// one's phase of the barrier for its own.  It knows of what the epilogue has finished, which is all up to b - 4.
+constexpr int kMinStages = 4;
+static_assert(kMinStages >= kMaxAcc, "an issuer knows of the box a ring before");
+constexpr size_t kWholeSm = 227 * 1024;          // what one CTA can have
+constexpr int kMostFused = 64;                   // blocks of k that a CTA keeps codes of
 constexpr int kBarBytes = 512;
 
 __device__ __forceinline__ void umma_f8_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -119,17 +125,38 @@ struct Shape {
     static constexpr int kTmem = NT * kAcc < 32 ? 32 : NT * kAcc;
     static constexpr int kABytes = NT * kFp8Block;               // a token box
     static constexpr int kPerSm = NT <= 32 ? 2 : 1;              // CTAs of an SM
-    static constexpr size_t kSmem = kPerSm == 2 ? 113 * 1024 : 227 * 1024;
+    static constexpr size_t kSmem = kPerSm == 2 ? 113 * 1024 : kWholeSm;
     static constexpr int kStage = kWBytes + (FUSED ? 0 : kABytes);
     // (after the ring: FUSED codes; sums from the cluster's CTAs [ranks][groups of tokens][128] x 4; slots of scales; FUSED scales)
     // groups of four tokens that one CTA of a cluster finishes, and what they take of its shared memory
-    static __host__ __device__ int share(int split) { return (NT / 4 + split - 1) / split; }
-    static __host__ __device__ int sum_floats(int split) { return share(split) * split * 4 * kRows; }
-    static size_t bytes(int stages, int split, int fused_blocks) {
+    static constexpr __host__ __device__ int share(int split) { return (NT / 4 + split - 1) / split; }
+    static constexpr __host__ __device__ int sum_floats(int split) { return share(split) * split * 4 * kRows; }
+    static constexpr size_t bytes(int stages, int split, int fused_blocks) {
         return 1024 + (size_t)stages * kStage + (FUSED ? (size_t)fused_blocks * (kABytes + NT * 4) : 0) + (split > 1 ? (size_t)sum_floats(split) * 4 : 0) +
                kAcc * NT * 4 + kBarBytes;
     }
+    // What a CTA gets that multiplies `mine` blocks of k: as long a ring as there is room for beside a second CTA, or, where that
+    // would be too short (FUSED with many blocks' codes to keep), with the SM to itself.
+    struct Fit {
+        int stages, per_sm;
+    };
+    static constexpr Fit fit(int split, int mine) {
+        const int fused_blocks = FUSED ? mine : 0;
+        const bool shared = bytes(kMinStages, split, fused_blocks) <= kSmem;
+        int stages = kMaxStages;
+        while (stages > kMinStages && bytes(stages, split, fused_blocks) > (shared ? kSmem : kWholeSm)) stages--;
+        return {stages, shared ? kPerSm : 1};
+    }
+    static constexpr bool always_fits() {
+        for (int split = 1; split <= kMaxSplit; split++)
+            for (int mine = 1; mine <= (kMostFused + split - 1) / split; mine++)
+                if (bytes(fit(split, mine).stages, split, FUSED ? mine : 0) > kWholeSm) return false;
+        return true;
+    }
 };
+static_assert(Shape<16, true>::always_fits() && Shape<16, false>::always_fits() && Shape<32, false>::always_fits() && Shape<64, false>::always_fits() &&
+                  Shape<128, false>::always_fits(),
+              "the shortest ring fits beside everything else");
 
 template <int NT, bool FUSED>
 __global__ void __launch_bounds__(Shape<NT, FUSED>::kThreads, (Shape<NT, FUSED>::kPerSm))
@@ -410,7 +437,7 @@ fp8_umma_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constan
 template <int NT, bool FUSED>
 cudaError_t prepare() {
     static PerDeviceOnce once;
-    return allow_dyn_smem(once, fp8_umma_kernel<NT, FUSED>, 227 * 1024);
+    return allow_dyn_smem(once, fp8_umma_kernel<NT, FUSED>, kWholeSm);
 }
 
 // Clusters of q CTAs that the device holds at a time (SMs are grouped, so eights and sevens leave some of them empty)
@@ -481,18 +508,15 @@ int launch(const uint8_t* codes, const uint8_t* w, Fp8Args a, int sm_count, cuda
     if (e != cudaSuccess) return -(int)e;
     const Plan plan = plan_for<NT, FUSED>(a.M, a.N, a.blocks, sm_count);
     const int split = plan.split;
-    const int fused_blocks = (a.blocks + split - 1) / split;
-    // FUSED with many blocks to a CTA: its codes leave room for two boxes beside a second CTA, or the SM is its own
-    size_t room = S::kSmem;
-    if (S::bytes(3, split, fused_blocks) > room) room = 227 * 1024;
-    a.stages = kMaxStages;
-    while (a.stages > 2 && S::bytes(a.stages, split, fused_blocks) > room) a.stages--;
-    const size_t smem = S::bytes(a.stages, split, fused_blocks);
+    const int mine = (a.blocks + split - 1) / split;
+    const typename S::Fit fit = S::fit(split, mine);
+    a.stages = fit.stages;
+    const size_t smem = S::bytes(a.stages, split, FUSED ? mine : 0);
     CUtensorMap map_w, map_a;
     if (!fp8_codes_map(&map_w, w, a.N, a.K, kRows) || (!FUSED && !fp8_codes_map(&map_a, codes, a.M, a.K, NT))) return -(int)cudaErrorInvalidValue;
     if (FUSED) map_a = map_w;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(split > 1 ? split * a.tiles : min(a.tiles, S::kPerSm * sm_count));
+    cfg.gridDim = dim3(split > 1 ? split * a.tiles : min(a.tiles, fit.per_sm * sm_count));
     cfg.blockDim = dim3(S::kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
@@ -511,7 +535,7 @@ int launch(const uint8_t* codes, const uint8_t* w, Fp8Args a, int sm_count, cuda
 }  // namespace
 
 // FUSED keeps the codes of sixteen rows in shared memory beside the weight ring
-bool fp8_fused_supported(int M, int K) { return M <= 16 && K <= 8192; }
+bool fp8_fused_supported(int M, int K) { return M <= 16 && K <= kMostFused * kFp8Block; }
 
 // In one kernel every CTA quantises all that it multiplies before its first product and keeps the codes; in two that is done once,
 // and the rings are longer.  The second launch costs the host 2.5 us, so two kernels are for where they save the GPU about that:

@@ -574,3 +574,22 @@ def test_rows_of_pairs_start_and_end_anywhere(moe, n, ld, offset, out):
     kept = torch.ones_like(buf, dtype=torch.bool)
     kept.as_strided((m, n), (ld, 1), storage_offset=offset).fill_(False)
     assert (buf[kept] == 77.0).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 40000, 2304), (16, 40000, 2816), (1, 40000, 2944), (3, 38000, 3200), (16, 40000, 3456), (1, 40000, 3840), (2, 40000, 3968),
+                                   (16, 38000, 5120), (1, 40000, 8176), (5, 40000, 8192), (2, 12800, 5120), (16, 12800, 5888), (1, 12800, 6656), (4, 9000, 6912),
+                                   (16, 9000, 7680), (1, 9000, 8192)])
+def test_one_kernel_with_many_blocks_to_a_cta(moe, m, n, k):
+    """Codes that leave the weight's ring little room, up to an SM for one CTA; whole and split over clusters."""
+    x = activations(m + k, m, k, torch.bfloat16).contiguous()
+    w, ws = weight(n + k, n, k)
+    two = torch.empty((m, n), device=DEV)
+    moe.fp8_gemm(*moe.fp8_quantize(x), w, ws, two)
+    lib, p, st, null = L.lib(), lambda t: C.c_void_p(t.data_ptr()), C.c_void_p(torch.cuda.current_stream().cuda_stream), C.c_void_p(0)
+    for _ in range(20):
+        c = torch.full((m + 1, n), 77.0, device=DEV)
+        assert lib.ftm_fp8_linear(moe._h, p(x), L.BF16, k, p(w), p(ws), m, n, k, null, null, p(c), L.F32, n, st) == L.OK
+        assert torch.equal(c[:m], two) and (c[m] == 77.0).all()
+    at = (n // 128 - 2) * 128
+    check_product(c[:m, at:], *quantised(x), w[at:], ws[at // 128:])
+    moe.sync_status()
