@@ -632,16 +632,25 @@ class B200MoE:
             return _current_stream()(self.device)
         return stream if isinstance(stream, int) else stream.cuda_stream
 
-    def _lend(self, tensors, on: int):
-        """Tensors made here for a call on stream `on`: where that is not the stream they were made on, their memory is not handed
-        out again before the call is done."""
+    def _make(self, on: int, device, kept: bool, *wanted):
+        """Tensors for a call on stream `on`, one for each (dtype, shape), None for None.  They come from that stream's own memory: a block that
+        another stream gave back may still be read there.  `kept`: the caller gets them and may use them on the current stream, which
+        then has to be done with them before the memory is handed out again."""
+        torch = _torch()
+
+        def new():
+            return [None if w is None else torch.empty(w[1], dtype=w[0], device=device) for w in wanted]
         on = on or self._own_stream
-        if on != _current_stream()(self.device):
-            torch = _torch()
-            there = torch.cuda.ExternalStream(on, device=self.device) if on else torch.cuda.default_stream(self.device)
-            for t in tensors:
+        if on == _current_stream()(self.device):
+            return new()
+        with torch.cuda.stream(torch.cuda.ExternalStream(on, device=self.device) if on else torch.cuda.default_stream(self.device)):
+            made = new()
+        if kept:
+            here = torch.cuda.current_stream(self.device)
+            for t in made:
                 if t is not None:
-                    t.record_stream(there)
+                    t.record_stream(here)
+        return made
 
     def _rows(self, t, what: str, codes: dict, shape=None) -> int:
         """Address of a matrix on this adapter's device whose last dimension is contiguous; its rows may be apart."""
@@ -672,7 +681,7 @@ class B200MoE:
         px = self._rows(x, "x", ty.act)
         m, k = x.shape
         on = self._on(stream)
-        q, scale = out = self._fp8_pair(x, m, k, on) if out is None else out
+        q, scale = out = self._fp8_pair(x, m, k, on, True) if out is None else out
         pq = self._flat(q, "the codes", ty.e4m3, (m, k))
         ps = self._flat(scale, "the scales", ty.f32, (-(-k // 128), m))
         rc = self._lib.ftm_fp8_quantize(self._h, px, ty.act[x.dtype], m, k, x.stride(0) if m > 1 else k, pq, ps, on)
@@ -701,7 +710,7 @@ class B200MoE:
         m, n, k, blocks, pw, pws, pc = self._fp8_operands(ty, x, w, w_scale, out)
         on = self._on(stream)
         if scratch is None and (m > 16 or k > 8192 or m * k > 20480 or (k > 2048 and m * k >= 8192)):
-            scratch = self._fp8_pair(x, m, k, on)
+            scratch = self._fp8_pair(x, m, k, on, False)
         pq = ps = None
         if scratch is not None:
             pq = self._flat(scratch[0], "the codes", ty.e4m3, (m, k))
@@ -712,13 +721,10 @@ class B200MoE:
             self._check(rc)
         return out
 
-    def _fp8_pair(self, x, m: int, k: int, on: int):
+    def _fp8_pair(self, x, m: int, k: int, on: int, kept: bool):
         """Room for the codes and scales of m rows of k, for a call on stream `on`."""
         torch = _torch()
-        made = (torch.empty((m, k), dtype=torch.float8_e4m3fn, device=x.device),
-                torch.empty((-(-k // 128), m), dtype=torch.float32, device=x.device))
-        self._lend(made, on)
-        return made
+        return tuple(self._make(on, x.device, kept, (torch.float8_e4m3fn, (m, k)), (torch.float32, (-(-k // 128), m))))
 
     def _fp8_operands(self, ty, a, w, w_scale, out):
         """Sizes and addresses that fp8_gemm and fp8_linear have in common."""
@@ -746,10 +752,9 @@ class B200MoE:
         on = self._on(stream)
         if out is None:
             torch = _torch()
-            new = lambda dtype, *shape: torch.empty(shape, dtype=dtype, device=logits.device)
-            out = (new(torch.float32, rows) if ids is not None else None, new(torch.float32, rows),
-                   new(torch.int32, rows) if ids is not None else None, new(torch.int32, rows, top_n), new(torch.float32, rows, top_n))
-            self._lend(out, on)
+            f32, i32, some = torch.float32, torch.int32, (rows, top_n)
+            out = tuple(self._make(on, logits.device, True, (f32, shape) if ids is not None else None, (f32, shape), (i32, shape) if ids is not None else None,
+                                   (i32, some), (f32, some)))
         lp, entropy, rank, top_ids, top_lp = out
         p1 = None if lp is None else flat(lp, "the log probabilities", ty.f32, shape)
         p2 = None if entropy is None else flat(entropy, "the entropies", ty.f32, shape)

@@ -593,3 +593,28 @@ def test_one_kernel_with_many_blocks_to_a_cta(moe, m, n, k):
     at = (n // 128 - 2) * 128
     check_product(c[:m, at:], *quantised(x), w[at:], ws[at // 128:])
     moe.sync_status()
+
+
+def test_memory_that_is_still_read_is_not_taken_for_another_stream(moe):
+    """A tensor of the scratch's or an output's size that was given back while a kernel of the current stream has yet to read it."""
+    m, n, k = 64, 256, 2048
+    x, (w, ws) = activations(1, m, k, torch.bfloat16), weight(2, n, k)
+    logits, ids = activations(3, 512, 300, torch.float32), torch.zeros(512, dtype=torch.int64, device=DEV)
+    side = torch.cuda.Stream()
+    want, c, lp = torch.empty((m, n), device=DEV), torch.empty((m, n), device=DEV), moe.logprobs(logits, ids, 4)
+    moe.fp8_linear(x, w, ws, want)
+    torch.cuda.synchronize()
+    sizes = [m * k, k // 128 * m * 4, 512 * 4, 512 * 16]
+    for given in (side, side.cuda_stream):
+        tensors = [torch.full((s,), 0x5a, dtype=torch.uint8, device=DEV) for s in sizes for _ in range(4)]
+        torch.cuda._sleep(50_000_000)
+        read = [t.clone() for t in tensors]
+        del tensors
+        moe.fp8_linear(x, w, ws, c, stream=given)
+        codes = moe.fp8_quantize(x, stream=given)
+        out = moe.logprobs(logits, ids, 4, stream=given)
+        torch.cuda.synchronize()
+        assert all((t == 0x5a).all() for t in read)
+        assert torch.equal(c, want) and codes[0].shape == (m, k)
+        for a, b in zip(out, lp):
+            assert torch.equal(a, b)

@@ -53,3 +53,54 @@ def test_reasons_name_what_is_wrong(moe, monkeypatch):
     refused(lambda: moe.logprobs(c, torch.zeros(3, dtype=torch.int64)), r"token ids is \(3,\)")
     refused(lambda: moe.logprobs(c, torch.zeros(4)), "token ids cannot be torch.float32")
     refused(lambda: moe.logprobs(c, None, 33), "at most 32")
+
+
+class Streams:
+    """Stands in for CUDA's streams and the library: notes the stream that each tensor is made on and each that is told of it."""
+
+    def __init__(self, monkeypatch, module):
+        self.now, self.made, self.told = 5, [], []
+        outer, empty = self, torch.empty
+
+        class Stream:
+            def __init__(self, handle, device=None):
+                self.handle = handle
+
+            def __enter__(self):
+                self.before, outer.now = outer.now, self.handle
+
+            def __exit__(self, *_):
+                outer.now = self.before
+
+        def noted(*a, **kw):
+            outer.made.append(outer.now)
+            return empty(*a, **kw)
+        monkeypatch.setattr(module, "_current_stream", lambda: lambda ordinal: outer.now)
+        monkeypatch.setattr(torch.cuda, "ExternalStream", Stream)
+        monkeypatch.setattr(torch.cuda, "stream", lambda s: s)
+        monkeypatch.setattr(torch.cuda, "default_stream", lambda device=None: Stream(0))
+        monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Stream(outer.now))
+        monkeypatch.setattr(torch, "empty", noted)
+        monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 0)
+        monkeypatch.setattr(torch.Tensor, "record_stream", lambda self, s: outer.told.append(s.handle))
+
+    def __getattr__(self, name):
+        return lambda *a: 0
+
+
+@pytest.mark.parametrize("given,own,on", [(9, 0, 9), (0, 0, 0), (0, 7, 7), (5, 0, 5), (0, 5, 5)])
+def test_what_a_call_makes_comes_from_the_stream_of_the_call(monkeypatch, given, own, on):
+    """From the current stream's memory it could be a block that is still read there.  5 is the current stream, 0 the default one or the
+    adapter's own."""
+    x, w, ws, c = torch.zeros((20, 256)), torch.zeros((130, 256), dtype=E4M3), torch.zeros((2, 2)), torch.zeros((20, 130))
+    ids = torch.zeros(20, dtype=torch.int64)
+    m = object.__new__(pkg.B200MoE)
+    streams = Streams(monkeypatch, importlib.import_module("ferrum-torrens_b200.moe"))
+    m._lib, m._h, m.device, m._own_stream = streams, None, 0, own
+    for call, tensors, kept in ((lambda: m.fp8_quantize(x, stream=given), 2, True), (lambda: m.fp8_linear(x, w, ws, c, stream=given), 2, False),
+                                (lambda: m.logprobs(c, ids, 3, stream=given), 5, True), (lambda: m.logprobs(c, None, stream=given), 3, True)):
+        streams.made.clear(), streams.told.clear()
+        call()
+        assert streams.made == [on] * tensors
+        # what the caller gets may be in use on the current stream when it is dropped
+        assert streams.told == ([5] * tensors if kept and on != 5 else [])
