@@ -625,7 +625,7 @@ class B200MoE:
 
     # -- block-scaled 8-bit products ------------------------------------------------------------
     # A decode step makes these calls by the hundred, and their kernels take a few microseconds: the checks below are one
-    # expression per tensor, and only a refusal looks for its reason.
+    # expression per tensor, and only a refusal looks for its reason.  (Sizes past 31 bits would be cut on the way to the library.)
     def _on(self, stream) -> int:
         """The stream of a call: the given one, else the current one of this adapter's device."""
         if stream is None:
@@ -680,6 +680,8 @@ class B200MoE:
         ty = _types()
         px = self._rows(x, "x", ty.act)
         m, k = x.shape
+        if (m | k) >> 31:
+            raise bad(f"fp8: {m} rows of {k} (at most 2^30 of either)")
         on = self._on(stream)
         q, scale = out = self._fp8_pair(x, m, k, on, True) if out is None else out
         pq = self._flat(q, "the codes", ty.e4m3, (m, k))
@@ -732,6 +734,8 @@ class B200MoE:
         if len(rows) != 2 or len(weight) != 2 or rows[1] != weight[1]:
             raise bad(f"fp8: a weight [N, K] is wanted for rows [M, K], got {tuple(weight)} for {tuple(rows)}")
         (m, k), n = rows, weight[0]
+        if (m | n | k) >> 31:
+            raise bad(f"fp8: {m} rows of {k} by {n} weight rows (at most 2^30 of each)")
         blocks = -(-k // 128)
         return (m, n, k, blocks, self._flat(w, "the weight", ty.e4m3, weight), self._flat(w_scale, "the weight's scales", ty.f32, (-(-n // 128), blocks)),
                 self._rows(out, "the output", ty.act, (m, n)))
@@ -745,6 +749,8 @@ class B200MoE:
         ty = _types()
         px = self._rows(logits, "the logits", ty.act)
         rows, vocab = logits.shape
+        if (rows | vocab) >> 31:
+            raise bad(f"logprobs: {rows} rows of {vocab} logits (less than 2^31 rows, at most 2^24 logits)")
         if not 0 <= top_n <= 32:
             raise bad(f"logprobs: {top_n} alternatives (at most 32)")
         flat, shape = self._flat, (rows,)

@@ -104,3 +104,19 @@ def test_what_a_call_makes_comes_from_the_stream_of_the_call(monkeypatch, given,
         assert streams.made == [on] * tensors
         # what the caller gets may be in use on the current stream when it is dropped
         assert streams.told == ([5] * tensors if kept and on != 5 else [])
+
+
+def test_sizes_past_32_bits_are_not_cut(moe, monkeypatch):
+    """The library takes sizes of 32 bits: what is larger would arrive there as another size, perhaps a valid one."""
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 0)
+    new = lambda dtype, *shape: torch.empty(shape, dtype=dtype, device="meta")
+    bf16, f32, i64, many = torch.bfloat16, torch.float32, torch.int64, 2 ** 32 + 16
+    refused(lambda: moe.fp8_quantize(new(bf16, many, 16), out=(new(E4M3, many, 16), new(f32, 1, many))), "2.30")
+    refused(lambda: moe.fp8_quantize(new(bf16, 2, many), out=(new(E4M3, 2, many), new(f32, many // 128 + 1, 2))), "2.30")
+    w, ws = new(E4M3, 8, 16), new(f32, 1, 1)
+    refused(lambda: moe.fp8_gemm(new(E4M3, many, 16), new(f32, 1, many), w, ws, new(f32, many, 8)), "2.30")
+    refused(lambda: moe.fp8_linear(new(bf16, many, 16), w, ws, new(f32, many, 8)), "2.30")
+    refused(lambda: moe.fp8_linear(new(bf16, 4, 16), new(E4M3, many, 16), new(f32, many // 128 + 1, 1), new(f32, 4, many)), "2.30")
+    refused(lambda: moe.fp8_linear(new(bf16, 4, many), new(E4M3, 8, many), new(f32, 1, many // 128 + 1), new(f32, 4, 8)), "2.30")
+    refused(lambda: moe.logprobs(new(bf16, many, 5), None), "2.24")
+    refused(lambda: moe.logprobs(new(f32, 3, many), new(i64, 3), out=(new(f32, 3), None, None, None, None)), "2.24")
