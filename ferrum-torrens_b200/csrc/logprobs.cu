@@ -626,6 +626,7 @@ logprobs_kernel(LogprobArgs a, int parts) {
             if (lane == 0) atomicExch(a.err, 3);
             return;
         }
+        __syncwarp();      // the list of every lane, before one lane reads it
     }
     uint64_t mine = best[lane];
     if (parts > 1 && n > 0) mine = merge_lists(lists, parts, n, lane);

@@ -54,3 +54,14 @@ def test_overlapped_kernels_promise_no_read_only_data_but_weights():
         bad = set(re.findall(r"const\s+[\w:]+\s*\*\s*__restrict__\s+(\w+)", params)) - weights
         assert not bad, (path, name, bad)
         assert "pdl_wait()" in body, (path, name)
+
+
+def _logprobs_body():
+    return next(body for _, name, _, body in _kernels() if name == "logprobs_kernel")
+
+
+def test_lists_of_lanes_are_ordered_before_one_lane_reads_them():
+    """Every lane stores its entry of the first list; the merge has one lane read them all."""
+    body = _logprobs_body()
+    between = body[body.index("lists[0][lane] ="):body.index("merge_lists(lists")]
+    assert "__syncwarp()" in between
