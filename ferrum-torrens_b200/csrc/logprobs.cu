@@ -623,6 +623,12 @@ logprobs_kernel(LogprobArgs a, int parts) {
         }
         lists[0][lane] = best[lane];
         if (!__all_sync(0xffffffffu, wait_for(bar, 0))) {
+            // Others may still be storing into this CTA: it stays until they have left the kernel (who has does not hold up the barrier;
+            // they wait for nothing any more) and, for about a millisecond, for what is on its way from them.
+            asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+            asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+            const long long from = clock64();
+            while (clock64() - from < 2000000) {}
             if (lane == 0) atomicExch(a.err, 3);
             return;
         }

@@ -65,3 +65,10 @@ def test_lists_of_lanes_are_ordered_before_one_lane_reads_them():
     body = _logprobs_body()
     between = body[body.index("lists[0][lane] ="):body.index("merge_lists(lists")]
     assert "__syncwarp()" in between
+
+
+def test_a_cta_that_gives_up_on_others_stays_until_they_are_done_with_its_memory():
+    body = _logprobs_body()
+    gave_up = body[body.index("wait_for(bar, 0)"):]
+    gave_up = gave_up[:gave_up.index("return;")]
+    assert "barrier.cluster.arrive" in gave_up and "clock64()" in gave_up[gave_up.index("barrier.cluster.wait"):]
