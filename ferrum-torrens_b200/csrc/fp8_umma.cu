@@ -498,6 +498,10 @@ Plan plan_for(int M, int N, int blocks, int sm_count) {
     return best;
 }
 
+// The same for pairs of SMs on tiles of 256 x 256, each of which takes `turns` of them.
+constexpr long long pair_ns(int blocks, long long turns) { return 6000 + 480ll * blocks * turns; }
+static_assert(pair_ns((1 << 30) / kFp8Block, 1) > 4000000000ll, "the most blocks there are");
+
 template <int NT, bool FUSED>
 int launch(const uint8_t* codes, const uint8_t* w, Fp8Args a, int sm_count, cudaStream_t s) {
     using S = Shape<NT, FUSED>;
@@ -565,7 +569,7 @@ int launch_fp8_gemm(const uint8_t* a, const float* a_scale, const uint8_t* w, co
         const long long pair_tiles = (long long)((M + 255) / 256) * ((N + 255) / 256), pairs = sm_count / 2;
         const long long ns32 = plan_for<32, false>(M, N, blocks, sm_count).ns, ns64 = plan_for<64, false>(M, N, blocks, sm_count).ns;
         const long long ns128 = M > 64 ? plan_for<128, false>(M, N, blocks, sm_count).ns : LLONG_MAX;
-        const long long ns_pair = M > 128 && pairs > 0 ? 6000 + 480 * blocks * ((pair_tiles + pairs - 1) / pairs) : LLONG_MAX;
+        const long long ns_pair = M > 128 && pairs > 0 ? pair_ns(blocks, (pair_tiles + pairs - 1) / pairs) : LLONG_MAX;
         const long long least = min(min(ns32, ns64), min(ns128, ns_pair));
         n = least == ns_pair ? launch_fp8_pair(a, a_scale, w, w_scale, M, N, K, out, out_dtype, ldc, sm_count, err, c.s)
             : least == ns128 ? launch<128, false>(a, w, g, sm_count, c.s)
