@@ -441,24 +441,24 @@ cudaError_t prepare() {
 }
 
 // Clusters of q CTAs that the device holds at a time (SMs are grouped, so eights and sevens leave some of them empty)
-template <int NT, bool FUSED>
+template <int NT>
 int clusters_at_once(int dev, int q) {
     static std::atomic<int> known[64][kMaxSplit + 1];
     if (dev < 0 || dev >= 64) return 0;
     int n = known[dev][q].load(std::memory_order_relaxed);
     if (n) return n;
-    if (prepare<NT, FUSED>() != cudaSuccess) return 0;
+    if (prepare<NT, false>() != cudaSuccess) return 0;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(q);
-    cfg.blockDim = dim3(Shape<NT, FUSED>::kThreads);
-    cfg.dynamicSmemBytes = Shape<NT, FUSED>::kSmem;
+    cfg.blockDim = dim3(Shape<NT, false>::kThreads);
+    cfg.dynamicSmemBytes = Shape<NT, false>::kSmem;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = q;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&n, fp8_umma_kernel<NT, FUSED>, &cfg) != cudaSuccess) {
+    if (cudaOccupancyMaxActiveClusters(&n, fp8_umma_kernel<NT, false>, &cfg) != cudaSuccess) {
         cudaGetLastError();
         n = 1;
     }
@@ -481,16 +481,17 @@ constexpr Costs kCosts = NT == 16   ? Costs{2200, 300, 300, 1800, 0}
                          : NT == 32 ? Costs{2200, 325, 210, 1900, 1000}
                          : NT == 64 ? Costs{2660, 345, 345, 2070, 0}
                                     : Costs{3400, 410, 410, 3000, 0};
-template <int NT, bool FUSED>
+// One plan for a size, whether the rows are quantised in the kernel or before it: the bits go by the split.
+template <int NT>
 Plan plan_for(int M, int N, int blocks, int sm_count) {
-    using S = Shape<NT, FUSED>;
+    using S = Shape<NT, false>;
     constexpr Costs c = kCosts<NT>;
     const long long tiles = (long long)((M + NT - 1) / NT) * ((N + kRows - 1) / kRows);
     Plan best{1, 0};
     int dev = -1;
     if (tiles * 2 <= S::kPerSm * sm_count && cudaGetDevice(&dev) != cudaSuccess) dev = -1;
     for (int q = 1; q <= kMaxSplit && q <= blocks && (q == 1 || tiles * q <= S::kPerSm * sm_count); q++) {
-        if (q > 1 && tiles > clusters_at_once<NT, FUSED>(dev, q)) continue;
+        if (q > 1 && tiles > clusters_at_once<NT>(dev, q)) continue;
         const long long each = (tiles * q + sm_count - 1) / sm_count, mine = (blocks + q - 1) / q;
         const long long ns = c.start + mine * (each > 1 ? c.several * each : c.alone) + (q > 1 ? c.join : 0) + (each > 1 ? c.second : 0);
         if (q == 1 || ns < best.ns) best = {q, ns};
@@ -510,7 +511,7 @@ int launch(const uint8_t* codes, const uint8_t* w, Fp8Args a, int sm_count, cuda
     a.tiles = a.t_tiles * ((a.N + kRows - 1) / kRows);
     cudaError_t e = prepare<NT, FUSED>();
     if (e != cudaSuccess) return -(int)e;
-    const Plan plan = plan_for<NT, FUSED>(a.M, a.N, a.blocks, sm_count);
+    const Plan plan = plan_for<NT>(a.M, a.N, a.blocks, sm_count);
     const int split = plan.split;
     const int mine = (a.blocks + split - 1) / split;
     const typename S::Fit fit = S::fit(split, mine);
@@ -548,7 +549,7 @@ bool fp8_fused_supported(int M, int K) { return M <= 16 && K <= kMostFused * kFp
 // 6.3, 6.4; 13 x 2048 x 4096 7.4, 6.6; 16 x 2048 x 8192 10.2, 8.2; two for 16 x 248320 x 2048 87.7, 84.9; 16 x 60000 x 2048
 // 29.3, 25.1; 3 x 40000 x 4096 43, 35; 2 x 20000 x 8192 55, 31.
 bool fp8_fused_faster(int M, int N, int K, int sm_count) {
-    const int blocks = (K + kFp8Block - 1) / kFp8Block, split = plan_for<16, true>(M, N, blocks, sm_count).split, mine = (blocks + split - 1) / split;
+    const int blocks = (K + kFp8Block - 1) / kFp8Block, split = plan_for<16>(M, N, blocks, sm_count).split, mine = (blocks + split - 1) / split;
     return mine <= 16 && mine * M <= 160;
 }
 
@@ -567,8 +568,8 @@ int launch_fp8_gemm(const uint8_t* a, const float* a_scale, const uint8_t* w, co
         // 100 x 8192 x 2048 9.5, 8.2, 9.8, -; 512 x 2048 x 2048 9.5, 8.2, 9.7, -; 200 x 8192 x 8192 52.5, 46.9, 29.9, 34.5; 256 x 8192 x 2048
         // 15.8, 14.1, 9.9, 12.8; 700 x 2048 x 4096 -, -, 16.6, 19.3; 400 x 5000 x 2048 -, -, 16.9, 13.0; 1000 x 8192 x 8192 177, 158, -, 68.
         const long long pair_tiles = (long long)((M + 255) / 256) * ((N + 255) / 256), pairs = sm_count / 2;
-        const long long ns32 = plan_for<32, false>(M, N, blocks, sm_count).ns, ns64 = plan_for<64, false>(M, N, blocks, sm_count).ns;
-        const long long ns128 = M > 64 ? plan_for<128, false>(M, N, blocks, sm_count).ns : LLONG_MAX;
+        const long long ns32 = plan_for<32>(M, N, blocks, sm_count).ns, ns64 = plan_for<64>(M, N, blocks, sm_count).ns;
+        const long long ns128 = M > 64 ? plan_for<128>(M, N, blocks, sm_count).ns : LLONG_MAX;
         const long long ns_pair = M > 128 && pairs > 0 ? pair_ns(blocks, (pair_tiles + pairs - 1) / pairs) : LLONG_MAX;
         const long long least = min(min(ns32, ns64), min(ns128, ns_pair));
         n = least == ns_pair ? launch_fp8_pair(a, a_scale, w, w_scale, M, N, K, out, out_dtype, ldc, sm_count, err, c.s)
