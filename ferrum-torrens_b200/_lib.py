@@ -62,6 +62,7 @@ _PROTOS = {
     "ftm_fp8_quantize": (_int, [_vp, _vp, _int, _i32, _i32, C.c_int64, _vp, _vp, _vp]),
     "ftm_fp8_gemm": (_int, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _int, C.c_int64, _vp]),
     "ftm_fp8_linear": (_int, [_vp, _vp, _int, C.c_int64, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _int, C.c_int64, _vp]),
+    "ftm_fp8_linear_scratch": (_int, [_vp, _i32, _i32, _i32]),
     "ftm_logprobs": (_int, [_vp, _vp, _int, _i32, _i32, C.c_int64, _vp, _int, _i32, _vp, _vp, _vp, _vp, _vp, _vp]),
     "ftm_ftw_open": (_int, [C.c_char_p, C.POINTER(_vp)]),
     "ftm_ftw_parse": (_int, [C.c_char_p, C.POINTER(_vp)]),

@@ -1321,6 +1321,16 @@ FTM_API int ftm_fp8_gemm(ftm_handle* h, const void* a_e4m3, const float* a_scale
                                              h->sm_count, h->flags + 2, h->ctx(pick(h, stream))), "fp8 gemm");
 }
 
+// Quantised inside the product's kernel where scratch for two is at hand?
+static bool fp8_in_one(const ftm_handle* h, int32_t m, int32_t n, int32_t k) { return fp8_fused_supported(m, k) && fp8_fused_faster(m, n, k, h->sm_count); }
+
+FTM_API int ftm_fp8_linear_scratch(ftm_handle* h, int32_t m, int32_t n, int32_t k) {
+    if (!h || m <= 0 || n <= 0 || k <= 0) return 0;
+    std::lock_guard<std::mutex> lk(h->mu);
+    DeviceGuard dg(h->cfg.ordinal);
+    return !fp8_in_one(h, m, n, k);
+}
+
 FTM_API int ftm_fp8_linear(ftm_handle* h, const void* x, int x_dtype, int64_t x_stride, const void* w_e4m3, const float* w_scale, int32_t m,
                            int32_t n, int32_t k, void* q_scratch, float* scale_scratch, void* c, int c_dtype, int64_t c_stride, void* stream) {
     if (!h) return FTM_ERR_BAD;
@@ -1332,7 +1342,7 @@ FTM_API int ftm_fp8_linear(ftm_handle* h, const void* x, int x_dtype, int64_t x_
     if (rc != FTM_OK) return rc;
     const Ctx ctx = h->ctx(pick(h, stream));
     const bool scratch = q_scratch && scale_scratch;
-    if (fp8_fused_supported(m, k) && (!scratch || fp8_fused_faster(m, n, k, h->sm_count)))
+    if (scratch ? fp8_in_one(h, m, n, k) : fp8_fused_supported(m, k))
         return count_launches(h, launch_fp8_linear(x, x_dtype, x_stride, (const uint8_t*)w_e4m3, w_scale, m, n, k, c, c_dtype, c_stride, h->sm_count,
                                                    h->flags + 2, ctx), "fp8 linear");
     if (!scratch) return fail(h, FTM_ERR_BAD, "moe: fp8 linear: %d rows of %d need scratch for their codes and scales", m, k);

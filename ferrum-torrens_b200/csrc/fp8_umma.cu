@@ -544,13 +544,15 @@ bool fp8_fused_supported(int M, int K) { return M <= 16 && K <= kMostFused * kFp
 
 // In one kernel every CTA quantises all that it multiplies before its first product and keeps the codes; in two that is done once,
 // and the rings are longer.  The second launch costs the host 2.5 us, so two kernels are for where they save the GPU about that:
-// more than 16 blocks of codes to a CTA (fewer than four weight boxes beside them) or more than 160 blocks of one row to quantise.
-// Rows x weight rows x k, us in one and in two kernels of a graph: one is taken for 1 x 248320 x 2048 79.7, 83.3; 8 x 2048 x 4096
-// 6.3, 6.4; 13 x 2048 x 4096 7.4, 6.6; 16 x 2048 x 8192 10.2, 8.2; two for 16 x 248320 x 2048 87.7, 84.9; 16 x 60000 x 2048
-// 29.3, 25.1; 3 x 40000 x 4096 43, 35; 2 x 20000 x 8192 55, 31.
+// more than 160 blocks of one row to quantise, or more than 16 blocks of codes to a CTA (fewer than four weight boxes beside them) unless
+// it has a dozen tiles to spread their quantisation over.
+// Rows x weight rows x k, us in one and in two kernels of a graph: one is taken for 1 x 248320 x 2048 79.6, 83.5; 8 x 2048 x 4096
+// 6.3, 6.4; 13 x 2048 x 4096 7.4, 6.6; 16 x 2048 x 8192 10.2, 8.2; 1 x 248320 x 4096 154, 162; 8 x 248320 x 2560 100, 105; 1 x 262144 x 2560 98, 107
+// (lost: 2 x 230000 x 6144 223, 215); two for 16 x 248320 x 2048 87.7, 84.9; 8 x 248320 x 4096 161, 159; 1 x 151936 x 4096 99, 100; 1 x 40000 x 4096
+// 37.0, 35.8; 3 x 40000 x 4096 37.7, 35.2; 1 x 60000 x 8176 96, 79; 16 x 60000 x 2048 29.4, 24.9; 2 x 20000 x 8192 51, 32.
 bool fp8_fused_faster(int M, int N, int K, int sm_count) {
     const int blocks = (K + kFp8Block - 1) / kFp8Block, split = plan_for<16>(M, N, blocks, sm_count).split, mine = (blocks + split - 1) / split;
-    return mine <= 16 && mine * M <= 160;
+    return mine * M <= 160 && (mine <= 16 || (N + kRows - 1) / kRows >= 12 * sm_count);
 }
 
 int launch_fp8_gemm(const uint8_t* a, const float* a_scale, const uint8_t* w, const float* w_scale, int M, int N, int K, void* out,

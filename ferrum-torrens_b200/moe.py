@@ -637,14 +637,11 @@ class B200MoE:
         another stream gave back may still be read there.  `kept`: the caller gets them and may use them on the current stream, which
         then has to be done with them before the memory is handed out again."""
         torch = _torch()
-
-        def new():
-            return [None if w is None else torch.empty(w[1], dtype=w[0], device=device) for w in wanted]
         on = on or self._own_stream
         if on == _current_stream()(self.device):
-            return new()
+            return [None if w is None else torch.empty(w[1], dtype=w[0], device=device) for w in wanted]
         with torch.cuda.stream(torch.cuda.ExternalStream(on, device=self.device) if on else torch.cuda.default_stream(self.device)):
-            made = new()
+            made = [None if w is None else torch.empty(w[1], dtype=w[0], device=device) for w in wanted]
         if kept:
             here = torch.cuda.current_stream(self.device)
             for t in made:
@@ -683,7 +680,10 @@ class B200MoE:
         if (m | k) >> 31:
             raise bad(f"fp8: {m} rows of {k} (at most 2^30 of either)")
         on = self._on(stream)
-        q, scale = out = self._fp8_pair(x, m, k, on, True) if out is None else out
+        if out is None:
+            torch = _torch()
+            out = tuple(self._make(on, x.device, True, (torch.float8_e4m3fn, (m, k)), (torch.float32, (-(-k // 128), m))))
+        q, scale = out
         pq = self._flat(q, "the codes", ty.e4m3, (m, k))
         ps = self._flat(scale, "the scales", ty.f32, (-(-k // 128), m))
         rc = self._lib.ftm_fp8_quantize(self._h, px, ty.act[x.dtype], m, k, x.stride(0) if m > 1 else k, pq, ps, on)
@@ -706,15 +706,19 @@ class B200MoE:
     def fp8_linear(self, x, w, w_scale, out, scratch=None, stream=None):
         """out [M, N] = fp8_gemm of fp8_quantize(x): x [M, K] bf16 or f32 (rows may be apart), the rest as for fp8_gemm.
         `scratch`: a pair as fp8_quantize returns it for x, kept by the caller, for the sizes that are faster in two kernels than
-        in one (made here when it is None and the rows are many or long)."""
+        in one (made here when it is None and the size is one of them)."""
         ty = _types()
         px = self._rows(x, "x", ty.act)
         m, n, k, blocks, pw, pws, pc = self._fp8_operands(ty, x, w, w_scale, out)
         on = self._on(stream)
-        if scratch is None and (m > 16 or k > 8192 or m * k > 20480 or (k > 2048 and m * k >= 8192)):
-            scratch = self._fp8_pair(x, m, k, on, False)
-        pq = ps = None
-        if scratch is not None:
+        # (sixteen blocks of k and no more than 160 of all rows never use it: the library is asked about the others)
+        if scratch is None and (m > 16 or ((blocks > 16 or m * blocks > 160) and self._lib.ftm_fp8_linear_scratch(self._h, m, n, k))):
+            room, = self._make(on, x.device, False, (_torch().uint8, (m * k + 4 * blocks * m,)))
+            pq = room.data_ptr()
+            ps = pq + m * k
+        elif scratch is None:
+            pq = ps = None
+        else:
             pq = self._flat(scratch[0], "the codes", ty.e4m3, (m, k))
             ps = self._flat(scratch[1], "the scales", ty.f32, (blocks, m))
         rc = self._lib.ftm_fp8_linear(self._h, px, ty.act[x.dtype], x.stride(0) if m > 1 else k, pw, pws, m, n, k, pq, ps, pc, ty.act[out.dtype],
@@ -722,11 +726,6 @@ class B200MoE:
         if rc:
             self._check(rc)
         return out
-
-    def _fp8_pair(self, x, m: int, k: int, on: int, kept: bool):
-        """Room for the codes and scales of m rows of k, for a call on stream `on`."""
-        torch = _torch()
-        return tuple(self._make(on, x.device, kept, (torch.float8_e4m3fn, (m, k)), (torch.float32, (-(-k // 128), m))))
 
     def _fp8_operands(self, ty, a, w, w_scale, out):
         """Sizes and addresses that fp8_gemm and fp8_linear have in common."""

@@ -276,10 +276,12 @@ FTM_API int ftm_fp8_gemm(ftm_handle* h, const void* a_e4m3, const float* a_scale
 /* ftm_fp8_gemm of ftm_fp8_quantize(x) in one call.  q_scratch [m, k] (16-byte aligned) and scale_scratch [ceil(k / 128), m] f32 are
  * the caller's, so calls that overlap on the GPU do not meet in them.  Up to 16 rows of up to 8192 elements can be one kernel,
  * which needs neither: they may be NULL then; given both, the call takes what is faster (many rows or long ones: two kernels).
- * The bits are the same.  Asynchronous. */
+ * The bits are the same.  Asynchronous.
+ * ftm_fp8_linear_scratch: 1 if a call of these sizes takes the scratch when it is given, 0 if it leaves it untouched. */
 FTM_API int ftm_fp8_linear(ftm_handle* h, const void* x, int x_dtype, int64_t x_stride, const void* w_e4m3, const float* w_scale,
                            int32_t m, int32_t n, int32_t k, void* q_scratch, float* scale_scratch, void* c, int c_dtype,
                            int64_t c_stride, void* stream);
+FTM_API int ftm_fp8_linear_scratch(ftm_handle* h, int32_t m, int32_t n, int32_t k);
 
 /* ---- what a server reads off its logits (no counterpart in the reference) ------------------------------------ */
 /* logits [rows, vocab] bf16 or f32 dev (vocab at most 2^24), rows row_stride elements apart (as ftm_dense_gemv or ftm_fp8_linear leave them);

@@ -618,3 +618,28 @@ def test_memory_that_is_still_read_is_not_taken_for_another_stream(moe):
         assert torch.equal(c, want) and codes[0].shape == (m, k)
         for a, b in zip(out, lp):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("sms", [0, 40])
+def test_scratch_is_made_where_two_kernels_are_taken(moe, sms):
+    """Given or not, the same kernels run: two where the library says that a size uses its scratch, else one."""
+    moe.set_sm_budget(sms)
+    try:
+        for m, n, k in [(1, 300, 16), (1, 40000, 2048), (1, 40000, 2064), (1, 40000, 4096), (1, 2048, 4096), (2, 20000, 4080), (2, 1000, 8192), (1, 60000, 8176),
+                        (3, 200, 2048), (10, 5000, 2048), (11, 5000, 2048), (16, 40000, 1280), (16, 40000, 1296), (16, 130, 1296), (13, 2048, 4096), (16, 64, 8192),
+                        (1, 64, 8208), (17, 64, 16), (40, 300, 256), (1, 230000, 2560), (8, 230000, 2560)]:
+            x, (w, ws) = activations(m, m, k, torch.bfloat16).contiguous(), weight(k, n, k)
+            scratch = moe.fp8_quantize(x)
+            c = torch.empty((2, m, n), device=DEV)
+            two = L.lib().ftm_fp8_linear_scratch(moe._h, m, n, k)
+            assert two in (0, 1) and (two == 1 or (m <= 16 and k <= 8192))
+            for i, given in enumerate((None, scratch)):
+                before = moe.kernel_launches()
+                moe.fp8_linear(x, w, ws, c[i], scratch=given)
+                assert moe.kernel_launches() - before == 1 + two, (m, n, k, given is None)
+            assert torch.equal(c[0], c[1])
+        for sizes in ((0, 1, 16), (1, 0, 16), (1, 1, 0), (-1, 5, 16)):
+            assert L.lib().ftm_fp8_linear_scratch(moe._h, *sizes) == 0
+        moe.sync_status()
+    finally:
+        moe.set_sm_budget(0)

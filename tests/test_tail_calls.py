@@ -97,7 +97,7 @@ def test_what_a_call_makes_comes_from_the_stream_of_the_call(monkeypatch, given,
     m = object.__new__(pkg.B200MoE)
     streams = Streams(monkeypatch, importlib.import_module("ferrum-torrens_b200.moe"))
     m._lib, m._h, m.device, m._own_stream = streams, None, 0, own
-    for call, tensors, kept in ((lambda: m.fp8_quantize(x, stream=given), 2, True), (lambda: m.fp8_linear(x, w, ws, c, stream=given), 2, False),
+    for call, tensors, kept in ((lambda: m.fp8_quantize(x, stream=given), 2, True), (lambda: m.fp8_linear(x, w, ws, c, stream=given), 1, False),
                                 (lambda: m.logprobs(c, ids, 3, stream=given), 5, True), (lambda: m.logprobs(c, None, stream=given), 3, True)):
         streams.made.clear(), streams.told.clear()
         call()
