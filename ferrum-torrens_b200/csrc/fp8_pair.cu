@@ -7,7 +7,7 @@
 // 256 x 256 x 32 by the first CTA into one of two accumulators that fill the tensor memory of both (512 cycles at the full rate).
 // As the scales change with the block, the epilogue warps read every accumulator back (128 lanes, one per token; two warps of
 // a quarter share its 256 columns, so each has one block of weight scales), multiply by one number per lane and add to 128
-// sums in registers, two per instruction, while the other accumulator is filled.
+// sums in registers while the other accumulator is filled.
 //   warp 0      TMA: this CTA's 128 token rows and 128 weight rows of a block; both CTAs' bytes count on the first one's barrier
 //   warps 1, 3  first CTA: issue the products of a block in turn and hand the stage and the accumulator over in both CTAs
 //   warp 2      fetches the scales of every block ahead of the epilogue

@@ -106,7 +106,6 @@ struct Word<float> {
     __device__ __forceinline__ static uint32_t reaching(const uint4& w, uint32_t v) {
         return any_reaches(w.x, v) | any_reaches(w.y, v) << 1 | any_reaches(w.z, v) << 2 | any_reaches(w.w, v) << 3;
     }
-    // how many elements of four words are above v, added to a tile's counts of even and odd elements
     // elements of a word that are v become -inf and are counted, in each half of `taken`
     __device__ __forceinline__ static void take_out(uint32_t& w, uint32_t v, uint32_t& taken) {
         if (__uint_as_float(w) == __uint_as_float(v)) w = kLowest, taken++;
@@ -117,6 +116,7 @@ struct Word<float> {
         asm("set.gt.f32.f32 %0, %1, %2;" : "=f"(r) : "f"(__uint_as_float(w)), "f"(v));
         return r;
     }
+    // how many elements of four words are above v, added to a tile's counts of even and odd elements
     __device__ __forceinline__ static void count_above(const uint4& w, uint32_t v, uint64_t& count) {
         const float f = __uint_as_float(v);
         count = add2(count, add2(pair(above(w.x, f), above(w.y, f)), pair(above(w.z, f), above(w.w, f))));

@@ -267,10 +267,10 @@ FTM_API int ftm_dense_gemv(ftm_handle* h, const void* a, int a_dtype, const void
 FTM_API int ftm_fp8_quantize(ftm_handle* h, const void* x, int x_dtype, int32_t rows, int32_t k, int64_t x_stride, void* q_e4m3,
                              float* scale, void* stream);
 /* c[t, n] = sum over blocks b of 128 k of  a_scale[b, t] * w_scale[n / 128, b] * sum_{k in b} a[t, k] * w[n, k],
- * every sum in f32, c rounded once.  a [m, k] and a_scale as ftm_fp8_quantize writes them; w [n, k] e4m3 dev and w_scale
- * [ceil(n / 128), ceil(k / 128)] f32 dev, the layout of checkpoints in 8 bits; a and w 16-byte aligned.  c [m, n] bf16 or
- * f32 dev, its rows c_stride elements apart (what lies between n and c_stride is not written).  k a multiple of 16; any m
- * and n from 1 on; each at most 2^30.  The same inputs give the same bits.  Asynchronous. */
+ * the product of the two scales (to stay in f32's normal range) and every sum in f32, c rounded once.  a [m, k] and a_scale as
+ * ftm_fp8_quantize writes them; w [n, k] e4m3 dev and w_scale [ceil(n / 128), ceil(k / 128)] f32 dev, the layout of checkpoints in
+ * 8 bits; a and w 16-byte aligned.  c [m, n] bf16 or f32 dev, its rows c_stride elements apart (what lies between n and c_stride is
+ * not written).  k a multiple of 16; any m and n from 1 on; each at most 2^30.  The same inputs give the same bits.  Asynchronous. */
 FTM_API int ftm_fp8_gemm(ftm_handle* h, const void* a_e4m3, const float* a_scale, const void* w_e4m3, const float* w_scale, int32_t m,
                          int32_t n, int32_t k, void* c, int c_dtype, int64_t c_stride, void* stream);
 /* ftm_fp8_gemm of ftm_fp8_quantize(x) in one call.  q_scratch [m, k] (16-byte aligned) and scale_scratch [ceil(k / 128), m] f32 are
