@@ -1325,7 +1325,7 @@ FTM_API int ftm_fp8_gemm(ftm_handle* h, const void* a_e4m3, const float* a_scale
 static bool fp8_in_one(const ftm_handle* h, int32_t m, int32_t n, int32_t k) { return fp8_fused_supported(m, k) && fp8_fused_faster(m, n, k, h->sm_count); }
 
 FTM_API int ftm_fp8_linear_scratch(ftm_handle* h, int32_t m, int32_t n, int32_t k) {
-    if (!h || m <= 0 || n <= 0 || k <= 0) return 0;
+    if (!h || m <= 0 || m > kMaxExtent || n <= 0 || n > kMaxExtent || k <= 0 || k > kMaxExtent || k % 16) return 0;
     std::lock_guard<std::mutex> lk(h->mu);
     DeviceGuard dg(h->cfg.ordinal);
     return !fp8_in_one(h, m, n, k);

@@ -544,7 +544,7 @@ bool fp8_fused_supported(int M, int K) { return M <= 16 && K <= kMostFused * kFp
 
 // In one kernel every CTA quantises all that it multiplies before its first product and keeps the codes; in two that is done once,
 // and the rings are longer.  The second launch costs the host 2.5 us, so two kernels are for where they save the GPU about that:
-// more than 160 blocks of one row to quantise, or more than 16 blocks of codes to a CTA (fewer than four weight boxes beside them) unless
+// more than 160 blocks of one row to quantise, or more than 16 blocks of codes to a CTA (the shortest ring beside them, or the SM to itself) unless
 // it has a dozen tiles to spread their quantisation over.
 // Rows x weight rows x k, us in one and in two kernels of a graph: one is taken for 1 x 248320 x 2048 79.6, 83.5; 8 x 2048 x 4096
 // 6.3, 6.4; 13 x 2048 x 4096 7.4, 6.6; 16 x 2048 x 8192 10.2, 8.2; 1 x 248320 x 4096 154, 162; 8 x 248320 x 2560 100, 105; 1 x 262144 x 2560 98, 107

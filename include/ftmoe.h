@@ -277,7 +277,7 @@ FTM_API int ftm_fp8_gemm(ftm_handle* h, const void* a_e4m3, const float* a_scale
  * the caller's, so calls that overlap on the GPU do not meet in them.  Up to 16 rows of up to 8192 elements can be one kernel,
  * which needs neither: they may be NULL then; given both, the call takes what is faster (many rows or long ones: two kernels).
  * The bits are the same.  Asynchronous.
- * ftm_fp8_linear_scratch: 1 if a call of these sizes takes the scratch when it is given, 0 if it leaves it untouched. */
+ * ftm_fp8_linear_scratch: 1 if a call of these sizes takes the scratch when it is given, 0 if it leaves it untouched (or refuses the sizes). */
 FTM_API int ftm_fp8_linear(ftm_handle* h, const void* x, int x_dtype, int64_t x_stride, const void* w_e4m3, const float* w_scale,
                            int32_t m, int32_t n, int32_t k, void* q_scratch, float* scale_scratch, void* c, int c_dtype,
                            int64_t c_stride, void* stream);

@@ -643,3 +643,11 @@ def test_scratch_is_made_where_two_kernels_are_taken(moe, sms):
         moe.sync_status()
     finally:
         moe.set_sm_budget(0)
+
+
+def test_scratch_of_sizes_that_are_refused(moe):
+    ask = lambda m, n, k: L.lib().ftm_fp8_linear_scratch(moe._h, m, n, k)
+    assert ask(17, 2 ** 30, 16) == 1 and ask(1, 64, 8208) == 1
+    for sizes in ((17, 2 ** 31 - 1, 16), (1, 2 ** 31 - 1, 8192), (1, 2 ** 30 + 1, 8192), (2 ** 30 + 1, 1, 16), (17, 64, 2 ** 30 + 16), (17, 64, 24), (17, 64, 8)):
+        assert ask(*sizes) == 0, sizes
+    assert L.lib().ftm_fp8_linear_scratch(C.c_void_p(0), 17, 64, 16) == 0
